@@ -299,6 +299,34 @@ int slim_attn_int8(const int8_t* q, const float* q_scale_t, const int8_t* k,
 int slim_attn_packed(const void* qkv, int64_t seq, int heads, int dim, int rotate, void* out,
                      void* workspace, uint64_t workspace_bytes, void* stream);
 
+/* ---------------------------------------------------------------- strided views
+ * Rows of `dim` consecutive elements addressed by (batch, token, head); strides in elements,
+ * 0 allowed for an input that is the same for every index of that dimension. */
+typedef struct slim_view {
+  void* data;
+  int64_t stride_b, stride_s, stride_h;
+} slim_view;
+
+/* ---------------------------------------------------------------- rotary positions */
+#define SLIM_ROTARY_HALF 0        /* pair j = elements j and j + rot/2 */
+#define SLIM_ROTARY_INTERLEAVED 1 /* pair j = elements 2j and 2j + 1 */
+#define SLIM_ROTARY_MAX_AXES 8
+
+/* Turn pair j of the first `rot` elements of every row of q (and of k, when heads_k > 0) by
+ * pos * inv_freq[j] (the opposite angle if inverse != 0), times magnitude; the other elements
+ * are passed through. q, q_out: [batch, seq, heads_q, dim]; k, k_out: [batch, seq, heads_k, dim],
+ * all of `dtype` (fp32 products and sums, one rounding). An output is its input itself (same data
+ * and strides) or does not overlap it. pos: 32- or 64-bit integers, element
+ * (b, s, axis) at b * pos_stride_b + s * pos_stride_s + axis * pos_stride_a; inv_freq: device
+ * fp32 [rot/2]. With axes > 1, sections (host, `axes` counts that add up to rot/2) gives the
+ * pairs of each axis in order. batch * seq < 2^31, dim <= 2048. */
+int slim_rotary(const slim_view* q, const slim_view* q_out, int heads_q, const slim_view* k,
+                const slim_view* k_out, int heads_k, int dtype, int64_t batch, int64_t seq,
+                int dim, int rot, int layout, const void* pos, int pos_bits,
+                int64_t pos_stride_b, int64_t pos_stride_s, int64_t pos_stride_a,
+                const float* inv_freq, const int* sections, int axes, float magnitude,
+                int inverse, void* stream);
+
 #ifdef __cplusplus
 }
 #endif

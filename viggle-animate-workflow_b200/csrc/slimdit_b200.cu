@@ -10,3 +10,4 @@
 #include "capi_nvfp4.cu"
 #include "verify.cu"
 #include "attn.cu"
+#include "rotary.cu"

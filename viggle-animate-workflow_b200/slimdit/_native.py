@@ -36,6 +36,14 @@ SLIM_ERR_NULL = -7
 F32, BF16, F16 = 0, 1, 2
 ORDER_REFERENCE, ORDER_BUTTERFLY = 0, 1
 EPI_SCALE_BIAS, EPI_GELU_TANH, EPI_SWIGLU = 0, 1, 2
+ROTARY_HALF, ROTARY_INTERLEAVED, ROTARY_MAX_AXES = 0, 1, 8
+
+
+class View(ctypes.Structure):
+    """slim_view: rows addressed by (batch, token, head), strides in elements."""
+
+    _fields_ = [("data", ctypes.c_void_p), ("stride_b", ctypes.c_int64), ("stride_s", ctypes.c_int64),
+                ("stride_h", ctypes.c_int64)]
 
 
 class NativeUnavailable(RuntimeError):
@@ -147,6 +155,12 @@ _SIGS = {
                                       ctypes.c_int, ctypes.c_int64, ctypes.c_void_p, ctypes.c_int64, ctypes.c_void_p]),
     "slim_attn_packed": (ctypes.c_int, [ctypes.c_void_p, ctypes.c_int64, ctypes.c_int, ctypes.c_int, ctypes.c_int,
                                         ctypes.c_void_p, ctypes.c_void_p, ctypes.c_uint64, ctypes.c_void_p]),
+    "slim_rotary": (ctypes.c_int, [ctypes.POINTER(View), ctypes.POINTER(View), ctypes.c_int, ctypes.POINTER(View),
+                                   ctypes.POINTER(View), ctypes.c_int, ctypes.c_int, ctypes.c_int64, ctypes.c_int64,
+                                   ctypes.c_int, ctypes.c_int, ctypes.c_int, ctypes.c_void_p, ctypes.c_int,
+                                   ctypes.c_int64, ctypes.c_int64, ctypes.c_int64, ctypes.c_void_p,
+                                   ctypes.POINTER(ctypes.c_int), ctypes.c_int, ctypes.c_float, ctypes.c_int,
+                                   ctypes.c_void_p]),
 }
 
 

@@ -17,6 +17,7 @@ computation runs in libslimdit_b200.so).
                     chunks overlapped on three streams
 * ``nvfp4_pack`` / ``nvfp4_quantize_act`` / ``nvfp4_dequantize`` / ``nvfp4_error`` /
   ``gemm_nvfp4`` / ``nvfp4_linear``  the NVFP4 format of slimdit/nvfp4.py and its linear
+* ``rotary``        rotary positions of queries and keys (frequencies: ``rope.rope_frequencies``)
 """
 
 from __future__ import annotations
@@ -517,3 +518,143 @@ def nvfp4_linear(x: torch.Tensor, qweight: torch.Tensor, block_scale: torch.Tens
                                                xs.data_ptr(), m, n, k, int(bool(rotate)), _EPI[epilogue], _stream(x2)))
     out = out.reshape(*lead, n)
     return out if out_dtype == torch.bfloat16 else out.to(out_dtype)
+
+
+# ---------------------------------------------------------------- rotary positions
+_LAYOUTS = {"half": nat.ROTARY_HALF, "interleaved": nat.ROTARY_INTERLEAVED}
+
+
+def _no_grad(*tensors) -> None:
+    """The kernels record no gradient: refuse tensors that expect one instead of dropping it."""
+    if torch.is_grad_enabled() and any(t is not None and t.requires_grad for t in tensors):
+        raise ValueError("this operator has no backward pass; call it under torch.no_grad() or detach its inputs")
+
+
+def _rows4(t: torch.Tensor, name: str, inplace: bool) -> torch.Tensor:
+    """[S, H, D] or [B, S, H, D] as a 4-D view with consecutive elements in each row."""
+    if not isinstance(t, torch.Tensor) or not t.is_cuda:
+        raise TypeError(f"{name} must be a CUDA tensor")
+    if t.dtype not in _DT:
+        raise TypeError(f"unsupported dtype {t.dtype}")
+    if t.dim() not in (3, 4):
+        raise ValueError(f"expected [tokens, heads, dim] or [batch, tokens, heads, dim] {name}, got {tuple(t.shape)}")
+    if t.dim() == 3:
+        t = t.unsqueeze(0)
+    if t.shape[3] > 1 and t.stride(3) != 1:
+        if inplace:
+            raise ValueError(f"{name} needs unit stride in its last dimension to be rotated in place")
+        t = t.contiguous()
+    return t
+
+
+def _view(t: torch.Tensor) -> nat.View:
+    st = t.stride()
+    return nat.View(t.data_ptr(), st[0], st[1], st[2])
+
+
+def _spans_overlap(t: torch.Tensor) -> bool:
+    """Whether two of the rows of t may share memory (every stride must step over what lies inside it)."""
+    reach = t.shape[3]
+    for size, stride in sorted(((n, s) for n, s in zip(t.shape[:3], t.stride()[:3]) if n > 1), key=lambda e: e[1]):
+        if stride < reach:
+            return True
+        reach += (size - 1) * stride
+    return False
+
+
+def _share(a: torch.Tensor, b: torch.Tensor) -> bool:
+    """Whether a row of a and a row of b may share memory: disjoint address ranges cannot, nor can two
+    column ranges of rows with one pitch (q and k of a packed buffer)."""
+    a0, b0 = a.data_ptr(), b.data_ptr()
+    size = a.element_size()
+    reach = [size * (1 + sum((n - 1) * s for n, s in zip(t.shape, t.stride()))) for t in (a, b)]
+    if a0 + reach[0] <= b0 or b0 + reach[1] <= a0:
+        return False
+    steps = [st * size for n, st, other in zip(a.shape[:2], a.stride(), b.stride()) if n > 1 and st == other]
+    if len(steps) != sum(n > 1 for n in a.shape[:2]) or not steps:
+        return True
+    pitch = min(steps)
+    if pitch <= 0 or any(st % pitch for st in steps):
+        return True
+    wide = [size * ((t.shape[2] - 1) * t.stride(2) + t.shape[3]) for t in (a, b)]
+    gap = (b0 - a0) % pitch
+    return gap < wide[0] or pitch - gap < wide[1]
+
+
+def rotary(q: torch.Tensor, k: torch.Tensor | None, positions: torch.Tensor, inv_freq: torch.Tensor,
+           layout: str = "half", sections=None, magnitude: float = 1.0, inverse: bool = False,
+           inplace: bool = False):
+    """Rotary positions of q and k in one launch: the first R = 2 * len(inv_freq) elements of every row
+    turn by position * frequency, the others pass through.
+
+    q: [B, S, H, D] or [S, H, D] (bf16/f16/f32 CUDA, any strides of the leading dimensions, e.g. the
+    views of a packed qkv buffer); k: the same with its own number of heads, or None. positions: int32
+    or int64, [S] or [B, S]; with ``sections`` (pairs of each position axis, in order, adding up to
+    R/2) [S, A] or [B, S, A]. inv_freq: fp32 [R/2], see :func:`slimdit.rope.rope_frequencies`, whose
+    magnitude is ``magnitude``. layout "half" pairs elements j and j + R/2, "interleaved" 2j and
+    2j + 1. ``inverse`` turns by the opposite angles (with 1/magnitude it undoes the rotation).
+    Returns (q', k'), or q' alone when k is None: new contiguous tensors, or q and k themselves with
+    ``inplace``. The angle is reduced in fp64, the products are fp32, rounded once."""
+    nat.require_cuda()
+    _no_grad(q, k)
+    if layout not in _LAYOUTS:
+        raise ValueError(f"layout must be one of {sorted(_LAYOUTS)}")
+    q4 = _rows4(q, "q", inplace)
+    b, s, h, d = q4.shape
+    dev = q4.device
+    k4 = None
+    if k is not None:
+        if isinstance(k, torch.Tensor) and k.dim() != q.dim():
+            raise ValueError("q and k must have the same number of dimensions")
+        k4 = _rows4(k, "k", inplace)
+        if k4.dtype != q4.dtype or k4.device != dev:
+            raise ValueError("q and k must have one dtype and one device")
+        if k4.shape[:2] != (b, s) or k4.shape[3] != d:
+            raise ValueError(f"k {tuple(k.shape)} does not fit q {tuple(q.shape)}")
+    if h == 0 or d == 0 or (k4 is not None and k4.shape[2] == 0):
+        raise ValueError("q and k need at least one head and one element")
+    if not isinstance(inv_freq, torch.Tensor) or inv_freq.dim() != 1:
+        raise ValueError("inv_freq must be a 1-D tensor")
+    if 2 * inv_freq.numel() > d or inv_freq.numel() == 0:
+        raise ValueError(f"{inv_freq.numel()} frequencies do not fit a head of {d} elements")
+    freq = inv_freq.to(device=dev, dtype=torch.float32).contiguous()
+    if not isinstance(positions, torch.Tensor) or positions.dtype not in (torch.int32, torch.int64):
+        raise TypeError("positions must be an int32 or int64 tensor")
+    if positions.device != dev:
+        raise ValueError("positions must be on the device of q")
+    axes = 1 if sections is None else len(sections)
+    if sections is not None and (not 1 <= axes <= nat.ROTARY_MAX_AXES or any(n < 0 for n in sections)
+                                 or sum(sections) != freq.numel()):
+        raise ValueError(f"sections {tuple(sections)} do not divide {freq.numel()} pairs")
+    shape = tuple(positions.shape) if sections is None else tuple(positions.shape[:-1])
+    if shape not in ((s,), (b, s), (1, s)) or (sections is not None and positions.shape[-1:] != (axes,)):
+        raise ValueError(f"positions {tuple(positions.shape)} do not fit {b} x {s} tokens and {axes} axes")
+    ps = positions.stride()
+    pos_a = ps[-1] if sections is not None else 0
+    pos_s = ps[len(shape) - 1]
+    pos_b = ps[0] if len(shape) == 2 and shape[0] == b and b > 1 else 0
+    if inplace:
+        for name, t in (("q", q4), ("k", k4)):
+            if t is not None and t.numel() and _spans_overlap(t):
+                raise ValueError(f"rows of {name} share memory: they cannot be rotated in place")
+        if k4 is not None and q4.numel() and _share(q4, k4):
+            raise ValueError("q and k may share memory: rotate them in place in two calls")
+        q_out, k_out = q4, k4
+    else:
+        q_out = torch.empty((b, s, h, d), dtype=q4.dtype, device=dev)
+        k_out = None if k4 is None else torch.empty(k4.shape, dtype=q4.dtype, device=dev)
+    qv, qo = _view(q4), _view(q_out)
+    kv, ko = (None, None) if k4 is None else (_view(k4), _view(k_out))
+    sec = None if sections is None else (nat.ctypes.c_int * axes)(*sections)
+    with torch.cuda.device(dev):
+        nat.check(nat.load().slim_rotary(qv, qo, h, kv, ko, 0 if k4 is None else k4.shape[2], _DT[q4.dtype], b, s, d,
+                                         2 * freq.numel(), _LAYOUTS[layout], positions.data_ptr(),
+                                         64 if positions.dtype == torch.int64 else 32, pos_b, pos_s, pos_a,
+                                         freq.data_ptr(), sec, axes, float(magnitude), int(bool(inverse)),
+                                         _stream(q4)))
+    if inplace:
+        return q if k is None else (q, k)
+    if q.dim() == 3:
+        q_out = q_out[0]
+        k_out = None if k_out is None else k_out[0]
+    return q_out if k is None else (q_out, k_out)
