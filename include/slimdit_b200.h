@@ -327,6 +327,28 @@ int slim_rotary(const slim_view* q, const slim_view* q_out, int heads_q, const s
                 const float* inv_freq, const int* sections, int axes, float magnitude,
                 int inverse, void* stream);
 
+/* ---------------------------------------------------------------- cross attention
+ * out = softmax(scale * q k^T + bias) v. q, out: [batch, q_len, heads, dim]; k, v: [batch, kv_len,
+ * kv_heads, dim] (heads a multiple of kv_heads, at most 128 to one), bf16 or fp16, rows 16-byte
+ * aligned; dim a multiple of 8 up to 128; k and v may have strides of 0. Scores, maxima and sums
+ * are fp32. */
+#define SLIM_MASK_BOOL 3 /* bytes: nonzero = the key takes part */
+
+/* Bytes of the workspace of slim_cross_attn; masked != 0 when a mask or lengths are given. */
+int slim_cross_attn_workspace_bytes(int64_t batch, int64_t q_len, int64_t kv_len, int heads,
+                                    int kv_heads, int dim, int masked, uint64_t* bytes);
+
+/* mask (or NULL): per key, element (b, i) at b * mask_stride_b + i * mask_stride_k; SLIM_MASK_BOOL
+ * or an additive SLIM_F32/BF16/F16 whose -inf excludes the key. kv_lengths (or NULL): device
+ * [batch] of 32- or 64-bit integers; keys from there on are excluded (clamped to 0..kv_len). What
+ * stands in excluded keys and values has no influence; a row without keys is 0. */
+int slim_cross_attn(const slim_view* q, const slim_view* k, const slim_view* v,
+                    const slim_view* out, int dtype, int64_t batch, int64_t q_len,
+                    int64_t kv_len, int heads, int kv_heads, int dim, const void* mask,
+                    int mask_type, int64_t mask_stride_b, int64_t mask_stride_k,
+                    const void* kv_lengths, int lengths_bits, float scale, void* workspace,
+                    uint64_t workspace_bytes, void* stream);
+
 #ifdef __cplusplus
 }
 #endif

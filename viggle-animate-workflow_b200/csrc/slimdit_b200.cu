@@ -11,3 +11,4 @@
 #include "verify.cu"
 #include "attn.cu"
 #include "rotary.cu"
+#include "cross_attn.cu"

@@ -36,6 +36,7 @@ SLIM_ERR_NULL = -7
 F32, BF16, F16 = 0, 1, 2
 ORDER_REFERENCE, ORDER_BUTTERFLY = 0, 1
 EPI_SCALE_BIAS, EPI_GELU_TANH, EPI_SWIGLU = 0, 1, 2
+MASK_BOOL = 3
 ROTARY_HALF, ROTARY_INTERLEAVED, ROTARY_MAX_AXES = 0, 1, 8
 
 
@@ -155,6 +156,14 @@ _SIGS = {
                                       ctypes.c_int, ctypes.c_int64, ctypes.c_void_p, ctypes.c_int64, ctypes.c_void_p]),
     "slim_attn_packed": (ctypes.c_int, [ctypes.c_void_p, ctypes.c_int64, ctypes.c_int, ctypes.c_int, ctypes.c_int,
                                         ctypes.c_void_p, ctypes.c_void_p, ctypes.c_uint64, ctypes.c_void_p]),
+    "slim_cross_attn_workspace_bytes": (ctypes.c_int, [ctypes.c_int64, ctypes.c_int64, ctypes.c_int64, ctypes.c_int,
+                                                       ctypes.c_int, ctypes.c_int, ctypes.c_int,
+                                                       ctypes.POINTER(ctypes.c_uint64)]),
+    "slim_cross_attn": (ctypes.c_int, [ctypes.POINTER(View), ctypes.POINTER(View), ctypes.POINTER(View),
+                                       ctypes.POINTER(View), ctypes.c_int, ctypes.c_int64, ctypes.c_int64,
+                                       ctypes.c_int64, ctypes.c_int, ctypes.c_int, ctypes.c_int, ctypes.c_void_p,
+                                       ctypes.c_int, ctypes.c_int64, ctypes.c_int64, ctypes.c_void_p, ctypes.c_int,
+                                       ctypes.c_float, ctypes.c_void_p, ctypes.c_uint64, ctypes.c_void_p]),
     "slim_rotary": (ctypes.c_int, [ctypes.POINTER(View), ctypes.POINTER(View), ctypes.c_int, ctypes.POINTER(View),
                                    ctypes.POINTER(View), ctypes.c_int, ctypes.c_int, ctypes.c_int64, ctypes.c_int64,
                                    ctypes.c_int, ctypes.c_int, ctypes.c_int, ctypes.c_void_p, ctypes.c_int,

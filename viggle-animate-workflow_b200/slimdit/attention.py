@@ -233,6 +233,91 @@ def attention_heads(qkv, heads: int, rank: int, world: int, rotate: bool = True,
     return out
 
 
+def _cross_rows(t, name: str):
+    """[S, H, D] or [B, S, H, D] as a 4-D view of 16-byte aligned rows (copied when it is not one)."""
+    import torch
+
+    if not isinstance(t, torch.Tensor) or not t.is_cuda:
+        raise TypeError(f"{name} must be a CUDA tensor")
+    if t.dtype not in (torch.bfloat16, torch.float16):
+        raise TypeError(f"cross attention takes bf16 or fp16 tensors, got {t.dtype} {name}")
+    if t.dim() not in (3, 4):
+        raise ValueError(f"expected [tokens, heads, dim] or [batch, tokens, heads, dim] {name}, got {tuple(t.shape)}")
+    if t.dim() == 3:
+        t = t.unsqueeze(0)
+    b, s, h, d = t.shape
+    st = t.stride()
+    if ((d > 1 and st[3] != 1) or t.data_ptr() % 16 or (b > 1 and st[0] % 8) or (s > 1 and st[1] % 8)
+            or (h > 1 and st[2] % 8)):
+        t = t.clone(memory_format=torch.contiguous_format)
+    return t
+
+
+def cross_attention(q, k, v, key_mask=None, kv_lengths=None, scale: float | None = None):
+    """softmax(scale * q k^T + bias) v of queries over the states of another sequence (an encoder's, a
+    prompt's) -> a new contiguous tensor of q's shape and dtype.
+
+    q: [B, Sq, H, D] or [Sq, H, D]; k, v: [B, Skv, Hkv, D] or [Skv, Hkv, D] with H a multiple of Hkv
+    (at most 128 heads to one), bf16 or fp16 CUDA, D a multiple of 8 up to 128. Any strides: rows that
+    are not 16-byte aligned or have gaps between their elements are copied first; k and v may be
+    expanded over the batch or the heads.
+    key_mask: [Skv] or [B, Skv] (or [B, 1, 1, Skv]), bool (True takes part) or additive fp32/bf16/fp16;
+    -inf excludes a key, a finite value, the type's lowest included, is added to its logits.
+    kv_lengths: int32 or int64 [B] on the device, keys from there on are excluded; with a mask both
+    apply. What stands in excluded keys and values, NaN included, has no influence; a row without keys
+    is 0. scale: D^-0.5 if not given. Scores, maxima and sums are fp32; the weights are rounded to the
+    type of v for the second product. Inference only: there is no backward pass."""
+    from . import _native as nat
+    from .ops import _no_grad, _view
+
+    torch = nat.require_cuda()
+    _no_grad(q, k, v, key_mask if isinstance(key_mask, torch.Tensor) else None)
+    q4, k4, v4 = _cross_rows(q, "q"), _cross_rows(k, "k"), _cross_rows(v, "v")
+    if k.dim() != q.dim() or v.dim() != q.dim():
+        raise ValueError("q, k and v must have the same number of dimensions")
+    b, sq, h, d = q4.shape
+    sk, hk = k4.shape[1:3]
+    dev = q4.device
+    if k4.dtype != q4.dtype or v4.dtype != q4.dtype or k4.device != dev or v4.device != dev:
+        raise ValueError("q, k and v must have one dtype and one device")
+    if k4.shape != v4.shape or k4.shape[0] != b or k4.shape[3] != d:
+        raise ValueError(f"k {tuple(k.shape)} and v {tuple(v.shape)} do not fit q {tuple(q.shape)}")
+    mask_type, mask_b, mask_k = 0, 0, 0
+    if key_mask is not None:
+        types = {torch.float32: nat.F32, torch.bfloat16: nat.BF16, torch.float16: nat.F16, torch.bool: nat.MASK_BOOL}
+        if not isinstance(key_mask, torch.Tensor) or key_mask.dtype not in types:
+            raise TypeError("key_mask must be a bool, fp32, bf16 or fp16 tensor")
+        if key_mask.device != dev:
+            raise ValueError("key_mask must be on the device of q")
+        m = key_mask[:, 0, 0] if key_mask.dim() == 4 and key_mask.shape[1:3] == (1, 1) else key_mask
+        if tuple(m.shape) not in ((sk,), (b, sk), (1, sk)):
+            raise ValueError(f"key_mask {tuple(key_mask.shape)} does not fit {b} x {sk} keys (masks per query are not "
+                             "supported)")
+        mask_type, mask_k = types[m.dtype], m.stride(-1)
+        mask_b = m.stride(0) if m.dim() == 2 and m.shape[0] == b and b > 1 else 0
+    if kv_lengths is not None:
+        if not isinstance(kv_lengths, torch.Tensor) or kv_lengths.dtype not in (torch.int32, torch.int64):
+            raise TypeError("kv_lengths must be an int32 or int64 tensor")
+        if kv_lengths.device != dev or tuple(kv_lengths.shape) != (b,):
+            raise ValueError(f"kv_lengths must be [{b}] on the device of q")
+        kv_lengths = kv_lengths.contiguous()
+    scale = max(d, 1) ** -0.5 if scale is None else float(scale)
+    lib = nat.load()
+    out = torch.empty((b, sq, h, d), dtype=q4.dtype, device=dev)
+    masked = key_mask is not None or kv_lengths is not None
+    need = ctypes.c_uint64(0)
+    with torch.cuda.device(dev):
+        nat.check(lib.slim_cross_attn_workspace_bytes(b, sq, sk, h, hk, d, int(masked), ctypes.byref(need)))
+        ws = torch.empty((need.value,), dtype=torch.uint8, device=dev) if need.value else None
+        nat.check(lib.slim_cross_attn(
+            _view(q4), _view(k4), _view(v4), _view(out), nat.BF16 if q4.dtype == torch.bfloat16 else nat.F16, b, sq, sk,
+            h, hk, d, None if key_mask is None else m.data_ptr(), mask_type, mask_b, mask_k,
+            None if kv_lengths is None else kv_lengths.data_ptr(),
+            0 if kv_lengths is None else 64 if kv_lengths.dtype == torch.int64 else 32, scale,
+            None if ws is None else ws.data_ptr(), need.value, torch.cuda.current_stream(dev).cuda_stream))
+    return out if q.dim() == 4 else out[0]
+
+
 @dataclasses.dataclass
 class TritonAttnConfig:
     """Settings of the attention override (the reference's name, attention_triton.py:225-245).
@@ -368,5 +453,5 @@ def install_triton_attn(config: TritonAttnConfig | None = None, stats: dict | No
 __all__ = [
     "DEFAULT_MIN_SEQ", "HEAD_DIM", "TritonAttnConfig", "TritonAttnOverride", "attention_heads", "attention_packed",
     "attention_quantized",
-    "attn_scale", "install_triton_attn", "packed_geometry", "quantized_operands", "unwrap", "workspace_bytes",
+    "attn_scale", "cross_attention", "install_triton_attn", "packed_geometry", "quantized_operands", "unwrap", "workspace_bytes",
 ]
