@@ -233,8 +233,9 @@ def attention_heads(qkv, heads: int, rank: int, world: int, rotate: bool = True,
     return out
 
 
-def _cross_rows(t, name: str):
-    """[S, H, D] or [B, S, H, D] as a 4-D view of 16-byte aligned rows (copied when it is not one)."""
+def _cross_rows(t, name: str, shared: bool):
+    """[S, H, D] or [B, S, H, D] as a 4-D view of 16-byte aligned rows (copied when it is not one);
+    ``shared``: strides of 0 may stay for the batch and the heads."""
     import torch
 
     if not isinstance(t, torch.Tensor) or not t.is_cuda:
@@ -248,7 +249,8 @@ def _cross_rows(t, name: str):
     b, s, h, d = t.shape
     st = t.stride()
     if ((d > 1 and st[3] != 1) or t.data_ptr() % 16 or (b > 1 and st[0] % 8) or (s > 1 and st[1] % 8)
-            or (h > 1 and st[2] % 8)):
+            or (h > 1 and st[2] % 8) or (s > 1 and st[1] == 0)
+            or (not shared and ((b > 1 and st[0] == 0) or (h > 1 and st[2] == 0)))):
         t = t.clone(memory_format=torch.contiguous_format)
     return t
 
@@ -272,7 +274,7 @@ def cross_attention(q, k, v, key_mask=None, kv_lengths=None, scale: float | None
 
     torch = nat.require_cuda()
     _no_grad(q, k, v, key_mask if isinstance(key_mask, torch.Tensor) else None)
-    q4, k4, v4 = _cross_rows(q, "q"), _cross_rows(k, "k"), _cross_rows(v, "v")
+    q4, k4, v4 = _cross_rows(q, "q", False), _cross_rows(k, "k", True), _cross_rows(v, "v", True)
     if k.dim() != q.dim() or v.dim() != q.dim():
         raise ValueError("q, k and v must have the same number of dimensions")
     b, sq, h, d = q4.shape
