@@ -334,9 +334,9 @@ int slim_rotary(const slim_view* q, const slim_view* q_out, int heads_q, const s
  * stride of 0 (shared by the sequences or heads). Scores, maxima and sums are fp32. */
 #define SLIM_MASK_BOOL 3 /* bytes: nonzero = the key takes part */
 
-/* Bytes of the workspace of slim_cross_attn; masked != 0 when a mask or lengths are given. */
+/* Bytes of the workspace of slim_cross_attn; additive != 0 when an additive mask is given. */
 int slim_cross_attn_workspace_bytes(int64_t batch, int64_t q_len, int64_t kv_len, int heads,
-                                    int kv_heads, int dim, int masked, uint64_t* bytes);
+                                    int kv_heads, int dim, int additive, uint64_t* bytes);
 
 /* mask (or NULL): per key, element (b, i) at b * mask_stride_b + i * mask_stride_k; SLIM_MASK_BOOL
  * or an additive SLIM_F32/BF16/F16 whose -inf excludes the key. kv_lengths (or NULL): device

@@ -24,27 +24,38 @@ constexpr float kLog2e = 1.4426950408889634f;
 constexpr int MAX_DIM = 128;
 constexpr int KEY_TILE = 128;
 
-enum MaskType : int { kMaskF32 = kF32, kMaskBF16 = kBF16, kMaskF16 = kF16, kMaskBool = 3, kMaskNone = -1 };
+
+// Which keys take part. A boolean mask and lengths are read by the attention kernel itself; an additive
+// mask goes through bias_kernel first (then lengths are in n_keys, and mask and lengths are null).
+struct Keys {
+  const uint8_t* mask;        // boolean mask or null
+  int64_t mask_b, mask_k;
+  const void* lengths;        // [batch] or null
+  int lengths64;
+  const float* bias;          // [batch, bias_pitch] base-2 bias per key, or null
+  int64_t bias_pitch;
+  const int* n_keys;          // [batch] keys in use (with bias), or null
+};
 
 struct Params {
   slim_view q, k, v, out;
   int64_t batch, q_len, kv_len;
   int heads, kv_heads, dim;
   float scale2;               // scale * log2 e
-  const float* bias;          // [batch, bias_pitch] base-2 bias per key, or null
-  int64_t bias_pitch;
-  const int* n_keys;          // [batch] keys in use (with bias), or null
+  Keys keys;
+  float* partial;             // split results (see split_floats), or null
 };
 
-// ---------------------------------------------------------------- mask -> base-2 bias per key
+__device__ __forceinline__ int64_t clamp_length(const void* lengths, int lengths64, int64_t b, int64_t kv_len) {
+  const int64_t l = lengths64 ? static_cast<const int64_t*>(lengths)[b] : static_cast<const int32_t*>(lengths)[b];
+  return l < 0 ? 0 : l < kv_len ? l : kv_len;
+}
+
+// ---------------------------------------------------------------- additive mask -> base-2 bias per key
 __device__ __forceinline__ float mask_value(const void* mask, int type, int64_t i) {
-  switch (type) {
-    case kMaskF32: return static_cast<const float*>(mask)[i];
-    case kMaskBF16: return __bfloat162float(static_cast<const __nv_bfloat16*>(mask)[i]);
-    case kMaskF16: return __half2float(static_cast<const __half*>(mask)[i]);
-    case kMaskBool: return static_cast<const uint8_t*>(mask)[i] ? 0.0f : -INFINITY;
-    default: return 0.0f;
-  }
+  if (type == kF32) return static_cast<const float*>(mask)[i];
+  if (type == kBF16) return __bfloat162float(static_cast<const __nv_bfloat16*>(mask)[i]);
+  return __half2float(static_cast<const __half*>(mask)[i]);
 }
 
 // One block per sequence: bias[b, i] = (mask[b, i] - max over the sequence) * log2 e, -inf for excluded
@@ -58,11 +69,7 @@ __global__ void __launch_bounds__(1024) bias_kernel(const void* __restrict__ mas
   __shared__ float s_max[32];
   __shared__ int s_last[32];
   const int64_t b = blockIdx.x;
-  int64_t len = kv_len;
-  if (lengths != nullptr) {
-    const int64_t l = lengths64 ? static_cast<const int64_t*>(lengths)[b] : static_cast<const int32_t*>(lengths)[b];
-    len = l < 0 ? 0 : l < kv_len ? l : kv_len;
-  }
+  const int64_t len = lengths != nullptr ? clamp_length(lengths, lengths64, b, kv_len) : kv_len;
   float top = -INFINITY;
   int last = 0;
   for (int64_t i = threadIdx.x; i < len; i += blockDim.x) {
@@ -102,16 +109,19 @@ __global__ void __launch_bounds__(1024) bias_kernel(const void* __restrict__ mas
 }
 
 // ---------------------------------------------------------------- tile kernel
-// One CTA takes 256 rows of one (sequence, key head): two tiles of 128 rows, a row being a (token,
-// query head of the group) pair with the head running fastest, so the heads that share keys share
-// their loads. 10 warps:
+// A row is a (token, query head of the group) pair, the head running fastest, so the heads that share
+// keys share their loads; 128 rows are a tile. Two tiles share a CTA, in one of two ways:
+//   wide   256 rows of one (sequence, key head), every key tile loaded once for both
+//   SPLIT  for few rows: one tile of rows, its keys cut over several CTAs and within a CTA over the
+//          two tiles (even and odd key tiles); partial sums go to memory and split_kernel joins them
+// 10 warps:
 //   warps 0..3, 4..7  softmax of tile 0 / 1, one row a thread: the scores are read from TMEM twice
 //                     (row maximum, then weights 2^(s scale2 + bias - m)), the weights go back packed
 //                     to 16 bits over the scores they came from, where the second product reads them.
 //                     O is rescaled only when a maximum grows by more than 2^8 over the one in use
 //                     (the weights stay below 2^8, sums and O are fp32), which is rare after the
 //                     first tile.
-//   warp 8            TMA: both Q tiles, then K_0 V_0 K_1 V_1 ... through one ring of tiles
+//   warp 8            TMA: the Q tiles, then key and value tiles in the order of their use, one ring
 //   warp 9            TMEM, and the MMAs: S_t = Q_t K_j^T, then per tile O_t += P_t V_j followed at
 //                     once by S_t = Q_t K_{j+1}^T: while one tile is in the softmax the tensor cores
 //                     work on the other.
@@ -124,13 +134,14 @@ __device__ __forceinline__ constexpr uint32_t col_s(int t) { return t * 128u; } 
 __device__ __forceinline__ constexpr uint32_t col_o(int t) { return 256u + t * 128u; }  // output accumulator
 constexpr float GROWTH = 8.0f;  // base-2 growth of a maximum that is let stand
 
-template <int DP>
+template <int DP, bool SPLIT>
 struct Layout {
   static constexpr int BLOCKS = DP / 64;               // 64-element (128-byte) column blocks of a tile
   static constexpr int BLOCK_BYTES = 128 * 128;
   static constexpr int TILE_BYTES = BLOCKS * BLOCK_BYTES;
-  static constexpr int STAGES = DP == 128 ? 5 : 8;
-  static constexpr int OFF_KV = 2 * TILE_BYTES;
+  static constexpr int Q_TILES = SPLIT ? 1 : 2;
+  static constexpr int STAGES = DP == 128 ? 7 - Q_TILES : 8;
+  static constexpr int OFF_KV = Q_TILES * TILE_BYTES;
   static constexpr int OFF_SH = OFF_KV + STAGES * TILE_BYTES;
 };
 
@@ -144,9 +155,9 @@ struct Shared {
   volatile int abort;
 };
 
-template <int DP>
+template <int DP, bool SPLIT>
 constexpr size_t smem_bytes() {
-  return 1024 + Layout<DP>::OFF_SH + sizeof(Shared<Layout<DP>::STAGES>);
+  return 1024 + Layout<DP, SPLIT>::OFF_SH + sizeof(Shared<Layout<DP, SPLIT>::STAGES>);
 }
 
 struct TileParams {
@@ -154,11 +165,20 @@ struct TileParams {
   int group, tokens;          // query heads per key head, tokens per 128-row tile
   int kb, kh, vb, vh;         // 0 for a k / v that is the same for every sequence / head
   float scale2;
-  const float* bias;
-  int64_t bias_pitch;
-  const int* n_keys;
+  Keys keys;
+  // SPLIT
+  int splits, per;            // CTAs per tile of rows, key tiles of each (even)
+  int rows;                   // rows of a tile that exist
+  float* partial;
 };
 
+// Partial results of `parts` pieces of `items` tiles of `rows` rows: (m, l) pairs, then O rows.
+__host__ __device__ inline int64_t split_floats(int64_t parts, int64_t items, int64_t rows, int dp) {
+  return parts * items * rows * (2 + dp);
+}
+
+__device__ __forceinline__ void store_f(__nv_bfloat16* p, float v) { *p = __float2bfloat16_rn(v); }
+__device__ __forceinline__ void store_f(__half* p, float v) { *p = __float2half_rn(v); }
 template <typename T>
 __device__ __forceinline__ uint32_t pack2(float lo, float hi);
 template <>
@@ -172,9 +192,9 @@ __device__ __forceinline__ uint32_t pack2<__half>(float lo, float hi) {
   return *reinterpret_cast<const uint32_t*>(&h);
 }
 
-// 32 scores of one row from TMEM as base-2 logits without the row's offset: s, or s scale2 + bias.
-template <bool MASK>
-__device__ __forceinline__ void load_scores(uint32_t taddr, int c, const float4* bias4, float scale2, int valid,
+// 32 scores of one row from TMEM: s where the bit is set and -inf elsewhere, or (BIAS) s scale2 + bias.
+template <bool BIAS>
+__device__ __forceinline__ void load_scores(uint32_t taddr, int c, const float4* bias4, float scale2, uint32_t bits,
                                             float (&y)[32]) {
   uint32_t r[32];
   tmem_ld_32x32b_x32(taddr + c, r);
@@ -182,7 +202,12 @@ __device__ __forceinline__ void load_scores(uint32_t taddr, int c, const float4*
   reg_dep32(r);
 #pragma unroll
   for (int e = 0; e < 32; ++e) y[e] = __uint_as_float(r[e]);
-  if (MASK) {
+  if (BIAS) {
+    if (bits == 0) {  // behind the last key: the bias row may end here
+#pragma unroll
+      for (int e = 0; e < 32; ++e) y[e] = -INFINITY;
+      return;
+    }
 #pragma unroll
     for (int e = 0; e < 32; e += 4) {
       const float4 b = __ldg(bias4 + (c + e) / 4);
@@ -192,17 +217,17 @@ __device__ __forceinline__ void load_scores(uint32_t taddr, int c, const float4*
       y[e + 2] = b.z == -INFINITY ? -INFINITY : fmaf(y[e + 2], scale2, b.z);
       y[e + 3] = b.w == -INFINITY ? -INFINITY : fmaf(y[e + 3], scale2, b.w);
     }
-  } else if (valid < BN) {
+  } else if (bits != 0xffffffffu) {
 #pragma unroll
-    for (int e = 0; e < 32; ++e) y[e] = c + e < valid ? y[e] : -INFINITY;
+    for (int e = 0; e < 32; ++e) y[e] = (bits >> e) & 1 ? y[e] : -INFINITY;
   }
 }
 
-template <typename T, int DP, bool MASK>
+template <typename T, int DP, bool BIAS, bool SPLIT>
 __global__ void __launch_bounds__(THREADS, 1)
 tile_kernel(const __grid_constant__ CUtensorMap tq, const __grid_constant__ CUtensorMap tk,
             const __grid_constant__ CUtensorMap tv, const __grid_constant__ CUtensorMap to, const TileParams p) {
-  using L = Layout<DP>;
+  using L = Layout<DP, SPLIT>;
   using Sh = Shared<L::STAGES>;
   constexpr bool BF16 = std::is_same<T, __nv_bfloat16>::value;
   constexpr uint32_t IDESC_QK = idesc_f16(BM, BN, BF16, false);
@@ -217,10 +242,21 @@ tile_kernel(const __grid_constant__ CUtensorMap tq, const __grid_constant__ CUte
   const int warp = threadIdx.x >> 5;
   const int lane = threadIdx.x & 31;
   const int b = blockIdx.z, hk = blockIdx.y;
-  const int64_t tok0 = static_cast<int64_t>(blockIdx.x) * 2 * p.tokens;
-  const int tiles = tok0 + p.tokens < p.q_len ? 2 : 1;
-  const int64_t keys = MASK ? p.n_keys[b] : p.kv_len;
+  const int split = SPLIT ? static_cast<int>(blockIdx.x % p.splits) : 0;
+  const int64_t q_tile = SPLIT ? blockIdx.x / p.splits : 2 * static_cast<int64_t>(blockIdx.x);
+  const int64_t tok0 = q_tile * p.tokens;
+  const int tiles = SPLIT || tok0 + p.tokens < p.q_len ? 2 : 1;
+  const int64_t keys = BIAS ? p.keys.n_keys[b]
+                       : p.keys.lengths != nullptr ? clamp_length(p.keys.lengths, p.keys.lengths64, b, p.kv_len)
+                                                   : p.kv_len;
+  // key tile of step j: wide, j for both tiles; SPLIT, j0 + 2 j + t
   const int nk = static_cast<int>((keys + BN - 1) / BN);
+  const int j0 = SPLIT ? split * p.per : 0;
+  const int steps = !SPLIT ? nk : nk <= j0 ? 0 : ((nk - j0 < p.per ? nk - j0 : p.per) + 1) / 2;
+  auto key_tile = [&](int t, int j) { return SPLIT ? j0 + 2 * j + t : j; };
+  // position of a tile's K and V of step j in the order of the loads
+  auto k_load = [](int t, int j) { return SPLIT ? 4 * j + t : 2 * j; };
+  auto v_load = [](int t, int j) { return SPLIT ? 4 * j + 2 + t : 2 * j + 1; };
 
   if (threadIdx.x == 0) {
     for (int t = 0; t < 2; ++t) {
@@ -248,38 +284,41 @@ tile_kernel(const __grid_constant__ CUtensorMap tq, const __grid_constant__ CUte
 
   if (warp == 8) {
     // ------------------------------------------------------------ TMA producer
-    if (lane == 0 && nk > 0) {
+    if (lane == 0 && steps > 0) {
       const uint32_t q_bytes = static_cast<uint32_t>(L::BLOCKS * 128 * p.group * p.tokens);
-      for (int t = 0; t < tiles; ++t) {
+      const int q_tiles = SPLIT ? 1 : tiles;
+      for (int t = 0; t < q_tiles; ++t) {
         mbar_arrive_expect_tx(&sh.q_full[t], q_bytes);
         for (int c = 0; c < L::BLOCKS; ++c)
           tma_load_4d(sQ + t * L::TILE_BYTES + c * L::BLOCK_BYTES, &tq, &sh.q_full[t], c * 64, hk * p.group,
                       static_cast<int32_t>(tok0 + t * p.tokens), b);
       }
       uint32_t issued = 0, last_parity = 0;
-      for (int i = 0; i < 2 * nk && !sh.abort; ++i) {  // K_0 V_0 K_1 V_1 ...
+      const int loads = (SPLIT ? 4 : 2) * steps;
+      for (int i = 0; i < loads && !sh.abort; ++i) {
         const int s = i % L::STAGES;
         const uint32_t ph = (i / L::STAGES) & 1;
         if (!mbar_wait(&sh.empty[s], ph ^ 1, kErrWaitTimeoutProducer)) {
           sh.abort = 1;
           break;
         }
-        const bool is_v = i & 1;
+        const bool is_v = SPLIT ? (i & 2) != 0 : (i & 1) != 0;
+        const int kt = SPLIT ? key_tile(i & 1, i >> 2) : i >> 1;
         mbar_arrive_expect_tx(&sh.full[s], L::TILE_BYTES);
-        for (int c = 0; c < L::BLOCKS; ++c)
+        for (int c = 0; c < L::BLOCKS; ++c)  // rows past the end come as zeros
           tma_load_4d(sKV + s * L::TILE_BYTES + c * L::BLOCK_BYTES, is_v ? &tv : &tk, &sh.full[s], c * 64,
-                      hk * (is_v ? p.vh : p.kh), (i >> 1) * BN, b * (is_v ? p.vb : p.kb));
+                      hk * (is_v ? p.vh : p.kh), kt * BN, b * (is_v ? p.vb : p.kb));
         issued |= 1u << s;
         last_parity = (last_parity & ~(1u << s)) | (ph << s);
       }
       // every load issued by this thread lands before the CTA may exit
-      for (int t = 0; t < tiles; ++t) mbar_wait(&sh.q_full[t], 0, kErrWaitTimeoutDrain);
+      for (int t = 0; t < q_tiles; ++t) mbar_wait(&sh.q_full[t], 0, kErrWaitTimeoutDrain);
       for (int s = 0; s < L::STAGES; ++s)
         if (issued & (1u << s)) mbar_wait(&sh.full[s], (last_parity >> s) & 1, kErrWaitTimeoutDrain);
     }
   } else if (warp == 9) {
     // ------------------------------------------------------------ MMA issue
-    if (lane == 0 && nk > 0) {
+    if (lane == 0 && steps > 0) {
       bool ok = true;
       auto wait = [&](uint64_t* bar, uint32_t parity) {
         ok = ok && mbar_wait(bar, parity, kErrWaitTimeoutMma) && !sh.abort;
@@ -287,7 +326,7 @@ tile_kernel(const __grid_constant__ CUtensorMap tq, const __grid_constant__ CUte
       };
       auto full = [&](int i) { return wait(&sh.full[i % L::STAGES], (i / L::STAGES) & 1); };
       auto qk = [&](int t, int i) {
-        const uint32_t qa = smem_u32(sQ + t * L::TILE_BYTES);
+        const uint32_t qa = smem_u32(sQ + (SPLIT ? 0 : t * L::TILE_BYTES));
         const uint32_t ka = smem_u32(sKV + (i % L::STAGES) * L::TILE_BYTES);
 #pragma unroll
         for (int k = 0; k < DP / 16; ++k) {
@@ -295,7 +334,7 @@ tile_kernel(const __grid_constant__ CUtensorMap tq, const __grid_constant__ CUte
           mma_f16(tmem + col_s(t), smem_desc_sw128(qa + off), smem_desc_sw128(ka + off), IDESC_QK, k != 0);
         }
         mma_commit(&sh.s_full[t]);
-        if (t == tiles - 1) mma_commit(&sh.empty[i % L::STAGES]);
+        if (SPLIT || t == tiles - 1) mma_commit(&sh.empty[i % L::STAGES]);
       };
       auto pv = [&](int t, int i, bool first) {
         const uint32_t va = smem_u32(sKV + (i % L::STAGES) * L::TILE_BYTES);
@@ -304,24 +343,22 @@ tile_kernel(const __grid_constant__ CUtensorMap tq, const __grid_constant__ CUte
           mma_f16_ta(tmem + col_o(t), tmem + col_s(t) + k * 8, smem_desc_mn_sw128(va + k * 2048, L::BLOCK_BYTES),
                      IDESC_PV, !(first && k == 0));
         mma_commit(&sh.o_full[t]);
-        if (t == tiles - 1) mma_commit(&sh.empty[i % L::STAGES]);
+        if (SPLIT || t == tiles - 1) mma_commit(&sh.empty[i % L::STAGES]);
       };
-      if (full(0)) {
-        for (int t = 0; t < tiles && wait(&sh.q_full[t], 0); ++t) {
-          tc_fence_after();
-          qk(t, 0);
-        }
+      for (int t = 0; t < tiles; ++t) {
+        if (!full(k_load(t, 0)) || !wait(&sh.q_full[SPLIT ? 0 : t], 0)) break;
+        tc_fence_after();
+        qk(t, k_load(t, 0));
       }
-      for (int j = 0; ok && j < nk; ++j) {
+      for (int j = 0; ok && j < steps; ++j) {
         for (int t = 0; t < tiles; ++t) {
-          if (t == 0 && !full(2 * j + 1)) break;
-          if (!wait(&sh.p_full[t], j & 1)) break;
+          if (!full(v_load(t, j)) || !wait(&sh.p_full[t], j & 1)) break;
           tc_fence_after();
-          pv(t, 2 * j + 1, j == 0);
-          if (j + 1 < nk) {
-            if (t == 0 && !full(2 * j + 2)) break;
+          pv(t, v_load(t, j), j == 0);
+          if (j + 1 < steps) {
+            if (!full(k_load(t, j + 1))) break;
             tc_fence_after();
-            qk(t, 2 * j + 2);
+            qk(t, k_load(t, j + 1));
           }
         }
       }
@@ -338,6 +375,8 @@ tile_kernel(const __grid_constant__ CUtensorMap tq, const __grid_constant__ CUte
     const uint32_t t_lane = tmem + (static_cast<uint32_t>(quarter * 32) << 16);
     const uint32_t t_s = t_lane + col_s(t), t_o = t_lane + col_o(t);
     const float scale2 = p.scale2;
+    // few rows: warps whose rows do not exist only keep step
+    const bool live = !SPLIT || quarter * 32 < p.rows;
     auto wait = [&](uint64_t* bar, uint32_t parity) {
       bool ok = mbar_wait(bar, parity, kErrWaitTimeoutEpilogue);
       ok = __all_sync(0xffffffffu, ok) && !sh.abort;
@@ -347,15 +386,31 @@ tile_kernel(const __grid_constant__ CUtensorMap tq, const __grid_constant__ CUte
     bool good = true;
     float m = -INFINITY;
     float2 l2 = make_float2(0.0f, 0.0f);
-    for (int j = 0; j < nk; ++j) {
-      const float4* bias4 = MASK ? reinterpret_cast<const float4*>(p.bias + b * p.bias_pitch + static_cast<int64_t>(j) * BN) : nullptr;
-      const int64_t left = keys - static_cast<int64_t>(j) * BN;
-      const int valid = left < BN ? static_cast<int>(left) : BN;
-      if (MASK && t == 0) {
-        // tile 0's weights gate the second product of both tiles
-        const bool clear = __ldg(reinterpret_cast<const float*>(bias4) + row) == -INFINITY;
+    for (int j = 0; j < steps; ++j) {
+      const int64_t key0 = static_cast<int64_t>(key_tile(t, j)) * BN;
+      const float4* bias4 = BIAS ? reinterpret_cast<const float4*>(p.keys.bias + b * p.keys.bias_pitch + key0) : nullptr;
+      // one bit per key of the tile that takes part (with a bias: per key up to the last one)
+      const int64_t left = keys - key0;
+      uint32_t bits[4];
+#pragma unroll
+      for (int w = 0; w < 4; ++w) {
+        const int64_t n = left - 32 * w;
+        bits[w] = n >= 32 ? 0xffffffffu : n <= 0 ? 0u : (1u << n) - 1u;
+      }
+      if (!BIAS && p.keys.mask != nullptr) {
+#pragma unroll
+        for (int w = 0; w < 4; ++w) {
+          const bool in = 32 * w + lane < left &&
+                          __ldg(p.keys.mask + b * p.keys.mask_b + (key0 + 32 * w + lane) * p.keys.mask_k) != 0;
+          bits[w] = __ballot_sync(0xffffffffu, in);
+        }
+      }
+      if (SPLIT || t == 0) {  // wide: tile 0's weights gate the second product of both tiles
+        const uint32_t mine = quarter == 0 ? bits[0] : quarter == 1 ? bits[1] : quarter == 2 ? bits[2] : bits[3];
+        bool clear = !((mine >> lane) & 1) && key0 + row < p.kv_len;
+        if (BIAS && !clear) clear = row < left && __ldg(reinterpret_cast<const float*>(bias4) + row) == -INFINITY;
         if (__any_sync(0xffffffffu, clear)) {
-          const int i = 2 * j + 1;
+          const int i = v_load(t, j);
           if (!(good = wait(&sh.full[i % L::STAGES], (i / L::STAGES) & 1))) break;
           if (clear) {
             uint4* v = reinterpret_cast<uint4*>(sKV + (i % L::STAGES) * L::TILE_BYTES + row * 128);
@@ -369,101 +424,130 @@ tile_kernel(const __grid_constant__ CUtensorMap tq, const __grid_constant__ CUte
       }
       if (!(good = wait(&sh.s_full[t], j & 1))) break;
       tc_fence_after();
-      float top = -INFINITY;
-#pragma unroll 1
-      for (int c = 0; c < BN; c += 32) {
-        float y[32];
-        load_scores<MASK>(t_s, c, bias4, scale2, valid, y);
-        float mx[4] = {y[0], y[1], y[2], y[3]};
+      if (live) {
+        float top = -INFINITY;
 #pragma unroll
-        for (int e = 4; e < 28; e += 8) {
+        for (int c = 0; c < BN; c += 32) {
+          float y[32];
+          load_scores<BIAS>(t_s, c, bias4, scale2, bits[c / 32], y);
+          float mx[4] = {y[0], y[1], y[2], y[3]};
 #pragma unroll
-          for (int u = 0; u < 4; ++u) mx[u] = fmax3(mx[u], y[e + u], y[e + 4 + u]);
+          for (int e = 4; e < 28; e += 8) {
+#pragma unroll
+            for (int u = 0; u < 4; ++u) mx[u] = fmax3(mx[u], y[e + u], y[e + 4 + u]);
+          }
+#pragma unroll
+          for (int u = 0; u < 4; ++u) mx[u] = fmaxf(mx[u], y[28 + u]);
+          top = fmaxf(top, fmaxf(fmax3(mx[0], mx[1], mx[2]), mx[3]));
         }
-#pragma unroll
-        for (int u = 0; u < 4; ++u) mx[u] = fmaxf(mx[u], y[28 + u]);
-        top = fmaxf(top, fmaxf(fmax3(mx[0], mx[1], mx[2]), mx[3]));
-      }
-      const float m_new = fmaxf(m, MASK ? top : top * scale2);
-      if (j == 0) {
-        m = m_new;
-      } else if (__any_sync(0xffffffffu, m_new > m + GROWTH)) {
-        const float alpha = m_new == -INFINITY ? 1.0f : ex2_approx(m - m_new);
-        m = m_new;
-        l2 = mul2(l2, make_float2(alpha, alpha));
-        if (!(good = wait(&sh.o_full[t], (j - 1) & 1))) break;
-        tc_fence_after();
+        const float m_new = fmaxf(m, BIAS ? top : top * scale2);
+        if (j == 0) {
+          m = m_new;
+        } else if (__any_sync(0xffffffffu, m_new > m + GROWTH)) {
+          const float alpha = m_new == -INFINITY ? 1.0f : ex2_approx(m - m_new);
+          m = m_new;
+          l2 = mul2(l2, make_float2(alpha, alpha));
+          if (!(good = wait(&sh.o_full[t], (j - 1) & 1))) break;
+          tc_fence_after();
 #pragma unroll 1
-        for (int c = 0; c < DP; c += 32) {
-          uint32_t r[32];
-          tmem_ld_32x32b_x32(t_o + c, r);
-          tmem_ld_wait();
-          reg_dep32(r);
+          for (int c = 0; c < DP; c += 32) {
+            uint32_t r[32];
+            tmem_ld_32x32b_x32(t_o + c, r);
+            tmem_ld_wait();
+            reg_dep32(r);
 #pragma unroll
-          for (int e = 0; e < 32; ++e) r[e] = __float_as_uint(__uint_as_float(r[e]) * alpha);
-          tmem_st_32x32b_x32(t_o + c, r);
+            for (int e = 0; e < 32; ++e) r[e] = __float_as_uint(__uint_as_float(r[e]) * alpha);
+            tmem_st_32x32b_x32(t_o + c, r);
+          }
         }
-      }
-      const float off = m == -INFINITY ? 0.0f : -m;
-      const float2 off2 = make_float2(off, off), sc2 = make_float2(scale2, scale2);
-#pragma unroll 1
-      for (int c = 0; c < BN; c += 32) {
-        float y[32];
-        load_scores<MASK>(t_s, c, bias4, scale2, valid, y);
-        uint32_t w[16];
+        const float off = m == -INFINITY ? 0.0f : -m;
+        const float2 off2 = make_float2(off, off), sc2 = make_float2(scale2, scale2);
 #pragma unroll
-        for (int e = 0; e < 16; ++e) {
-          const float2 a = make_float2(y[2 * e], y[2 * e + 1]);
-          const float2 x = MASK ? add2(a, off2) : fma2(a, sc2, off2);
-          const float2 g = make_float2(ex2_approx(x.x), ex2_approx(x.y));
-          l2 = add2(l2, g);
-          w[e] = pack2<T>(g.x, g.y);
+        for (int c = 0; c < BN; c += 32) {
+          float y[32];
+          load_scores<BIAS>(t_s, c, bias4, scale2, bits[c / 32], y);
+          uint32_t w[16];
+#pragma unroll
+          for (int e = 0; e < 16; ++e) {
+            const float2 a = make_float2(y[2 * e], y[2 * e + 1]);
+            const float2 x = BIAS ? add2(a, off2) : fma2(a, sc2, off2);
+            const float2 g = make_float2(ex2_approx(x.x), ex2_approx(x.y));
+            l2 = add2(l2, g);
+            w[e] = pack2<T>(g.x, g.y);
+          }
+          tmem_st_32x32b_x16(t_s + c / 2, w);
         }
-        tmem_st_32x32b_x16(t_s + c / 2, w);
+        tmem_st_wait();
       }
-      tmem_st_wait();
       tc_fence_before();
       mbar_arrive(&sh.p_full[t]);
     }
-    // the tile's rows leave through the shared memory of its queries
-    uint8_t* stage = sQ + t * L::TILE_BYTES;
     const float l = l2.x + l2.y;
-    if (good && nk > 0) {
-      good = wait(&sh.o_full[t], (nk - 1) & 1);
+    if (good && steps > 0) {
+      good = wait(&sh.o_full[t], (steps - 1) & 1);
       tc_fence_after();
     }
-    if (good) {
-      const float inv = l == 0.0f ? 0.0f : 1.0f / l;
+    if (SPLIT) {
+      // (m, l) and O of this piece; O stays unwritten where no key took part
+      if (good && !sh.abort && live) {
+        const int64_t items = static_cast<int64_t>(gridDim.x / p.splits) * gridDim.y * gridDim.z;
+        const int64_t item = (static_cast<int64_t>(b) * gridDim.y + hk) * (gridDim.x / p.splits) + q_tile;
+        const int64_t at = ((2 * split + t) * items + item) * p.rows + row;
+        const int64_t parts = 2 * p.splits;
+        const bool exists = row < p.rows;
+        if (exists) reinterpret_cast<float2*>(p.partial)[at] = make_float2(m, l);
+        if (steps > 0) {
+          float* o = p.partial + 2 * parts * items * p.rows + at * DP;
 #pragma unroll 1
-      for (int c = 0; c < DP; c += 32) {
-        uint32_t r[32];
-        if (nk > 0) {
-          tmem_ld_32x32b_x32(t_o + c, r);
-          tmem_ld_wait();
-          reg_dep32(r);
-        } else {
+          for (int c = 0; c < DP; c += 32) {
+            uint32_t r[32];
+            tmem_ld_32x32b_x32(t_o + c, r);
+            tmem_ld_wait();
+            reg_dep32(r);
+            if (exists) {
 #pragma unroll
-          for (int e = 0; e < 32; ++e) r[e] = 0;
-        }
-        uint8_t* dst = stage + (c >> 6) * L::BLOCK_BYTES + row * 128;
-#pragma unroll
-        for (int u = 0; u < 4; ++u) {
-          uint32_t w[4];
-#pragma unroll
-          for (int e = 0; e < 4; ++e)
-            w[e] = pack2<T>(__uint_as_float(r[8 * u + 2 * e]) * inv, __uint_as_float(r[8 * u + 2 * e + 1]) * inv);
-          const int chunk = ((c & 63) >> 3) + u;
-          *reinterpret_cast<uint4*>(dst + ((chunk ^ (row & 7)) << 4)) = make_uint4(w[0], w[1], w[2], w[3]);
+              for (int u = 0; u < 8; ++u)
+                reinterpret_cast<uint4*>(o + c)[u] = make_uint4(r[4 * u], r[4 * u + 1], r[4 * u + 2], r[4 * u + 3]);
+            }
+          }
         }
       }
-      fence_proxy_async_smem();
-    }
-    named_barrier(1 + t, BM);  // reached on every path
-    if (good && !sh.abort && quarter == 0 && lane == 0) {
-      for (int c = 0; c < L::BLOCKS; ++c)
-        tma_store_4d(&to, stage + c * L::BLOCK_BYTES, c * 64, hk * p.group, static_cast<int32_t>(tok0 + t * p.tokens), b);
-      bulk_commit_group();
-      bulk_wait_group<0>();
+    } else {
+      // the tile's rows leave through the shared memory of its queries
+      uint8_t* stage = sQ + t * L::TILE_BYTES;
+      if (good) {
+        const float inv = l == 0.0f ? 0.0f : 1.0f / l;
+#pragma unroll 1
+        for (int c = 0; c < DP; c += 32) {
+          uint32_t r[32];
+          if (steps > 0) {
+            tmem_ld_32x32b_x32(t_o + c, r);
+            tmem_ld_wait();
+            reg_dep32(r);
+          } else {
+#pragma unroll
+            for (int e = 0; e < 32; ++e) r[e] = 0;
+          }
+          uint8_t* dst = stage + (c >> 6) * L::BLOCK_BYTES + row * 128;
+#pragma unroll
+          for (int u = 0; u < 4; ++u) {
+            uint32_t w[4];
+#pragma unroll
+            for (int e = 0; e < 4; ++e)
+              w[e] = pack2<T>(__uint_as_float(r[8 * u + 2 * e]) * inv, __uint_as_float(r[8 * u + 2 * e + 1]) * inv);
+            const int chunk = ((c & 63) >> 3) + u;
+            *reinterpret_cast<uint4*>(dst + ((chunk ^ (row & 7)) << 4)) = make_uint4(w[0], w[1], w[2], w[3]);
+          }
+        }
+        fence_proxy_async_smem();
+      }
+      named_barrier(1 + t, BM);  // reached on every path
+      if (good && !sh.abort && quarter == 0 && lane == 0) {
+        for (int c = 0; c < L::BLOCKS; ++c)
+          tma_store_4d(&to, stage + c * L::BLOCK_BYTES, c * 64, hk * p.group, static_cast<int32_t>(tok0 + t * p.tokens), b);
+        bulk_commit_group();
+        bulk_wait_group<0>();
+      }
     }
   }
   tc_fence_before();
@@ -471,6 +555,59 @@ tile_kernel(const __grid_constant__ CUtensorMap tq, const __grid_constant__ CUte
   if (warp == 9) {
     tc_fence_after();
     tmem_dealloc(tmem, 512);
+  }
+}
+
+// ---------------------------------------------------------------- joining the pieces of a split
+// One block per row: 8 warps take every 8th piece, a lane DP / 32 columns; pieces in a fixed order.
+// out = sum_i 2^(m_i - M) O_i / sum_i 2^(m_i - M) l_i, pieces without keys left unread.
+template <typename T, int DP>
+__global__ void __launch_bounds__(256) split_kernel(const float* __restrict__ partial, slim_view out, int64_t q_len,
+                                                    int group, int tokens, int rows, int q_tiles, int kv_heads,
+                                                    int parts, int64_t items, int dim) {
+  constexpr int E = DP / 32;
+  __shared__ float s_o[8][DP];
+  __shared__ float s_l[8], s_m[8];
+  const int lane = threadIdx.x & 31, warp = threadIdx.x >> 5;
+  const int64_t item = blockIdx.x / rows;
+  const int row = static_cast<int>(blockIdx.x - item * rows);
+  const int64_t token = item % q_tiles * tokens + row / group;
+  if (token >= q_len) return;  // whole blocks
+  const float2* ml = reinterpret_cast<const float2*>(partial) + item * rows + row;
+  const float* o = partial + 2 * parts * items * rows + (item * rows + row) * DP + lane * E;
+  const int64_t step = items * rows;
+  float top = -INFINITY;
+  for (int i = lane; i < parts; i += 32) top = fmaxf(top, ml[i * step].x);
+#pragma unroll
+  for (int sft = 16; sft >= 1; sft >>= 1) top = fmaxf(top, __shfl_xor_sync(0xffffffffu, top, sft));
+  const float off = top == -INFINITY ? 0.0f : top;
+  float acc[E] = {}, l = 0.0f;
+#pragma unroll 4
+  for (int i = warp; i < parts; i += 8) {
+    const float2 a = ml[i * step];
+    if (a.y == 0.0f) continue;
+    const float w = exp2f(a.x - off);
+    l = fmaf(w, a.y, l);
+#pragma unroll
+    for (int e = 0; e < E; ++e) acc[e] = fmaf(w, o[i * step * DP + e], acc[e]);
+  }
+#pragma unroll
+  for (int e = 0; e < E; ++e) s_o[warp][lane * E + e] = acc[e];
+  if (lane == 0) s_l[warp] = l;
+  __syncthreads();
+  const int d = threadIdx.x;
+  if (d < dim) {
+    float x = 0.0f;
+    l = 0.0f;
+#pragma unroll
+    for (int w = 0; w < 8; ++w) {
+      x += s_o[w][d];
+      l += s_l[w];
+    }
+    const int64_t b = item / q_tiles / kv_heads;
+    const int h = static_cast<int>(item / q_tiles % kv_heads) * group + row % group;
+    T* dst = static_cast<T*>(out.data) + b * out.stride_b + token * out.stride_s + h * out.stride_h;
+    store_f(dst + d, l == 0.0f ? 0.0f : x / l);
   }
 }
 
@@ -494,54 +631,103 @@ static bool make_map(CUtensorMap* map, bool bf16, const slim_view& v, int64_t ba
              CU_TENSOR_MAP_FLOAT_OOB_FILL_NONE) == CUDA_SUCCESS;
 }
 
-template <typename T, int DP, bool MASK>
-cudaError_t launch(const Params& p, cudaStream_t st) {
+// How a problem is laid over the SMs: splits = 0 for the wide form.
+struct Plan {
+  int group, tokens;
+  int64_t q_tiles;
+  int splits, per;            // per: key tiles of a split, even
+  int rows;
+  int64_t floats;             // of partial results
+};
+
+// The wide form takes 2 row tiles x key tiles steps per CTA; SPLIT 1 row tile x 2 key tiles a step, more
+// CTAs, and a second launch. Costs in steps (about 2.5 us): a wave of CTAs has to start and end (2), the
+// join costs 1.5. The cheapest wins: with few rows SPLIT, with many waves of CTAs the wide form.
+inline Plan make_plan(int64_t batch, int64_t q_len, int64_t kv_len, int heads, int kv_heads, int dim) {
+  Plan p{};
+  p.group = heads / kv_heads;
+  p.tokens = BM / p.group;
+  p.q_tiles = (q_len + p.tokens - 1) / p.tokens;
+  const int64_t nk = (kv_len + BN - 1) / BN, base = batch * kv_heads, sms = sm_count();
+  auto waves = [&](int64_t ctas) { return (ctas + sms - 1) / sms; };
+  double best = static_cast<double>(waves(base * ((p.q_tiles + 1) / 2))) * (2.0 + static_cast<double>(nk));
+  for (int64_t s = 1; s <= 64 && 2 * (s - 1) < nk; ++s) {
+    const int64_t per = (nk + 2 * s - 1) / (2 * s) * 2;
+    if ((s - 1) * per >= nk) continue;  // the last CTAs would have nothing
+    const double cost = static_cast<double>(waves(base * p.q_tiles * s)) * (2.0 + static_cast<double>(per) / 2) + 1.5;
+    if (cost < best && base * p.q_tiles * s < (int64_t{1} << 24)) {
+      best = cost;
+      p.splits = static_cast<int>(s);
+      p.per = static_cast<int>(per);
+    }
+  }
+  if (p.splits > 0) {
+    p.rows = p.group * static_cast<int>(q_len < p.tokens ? q_len : p.tokens);
+    p.floats = split_floats(2 * p.splits, base * p.q_tiles, p.rows, dim > 64 ? 128 : 64);
+  }
+  return p;
+}
+
+template <typename T, int DP, bool BIAS, bool SPLIT>
+cudaError_t launch(const Params& p, const Plan& plan, cudaStream_t st) {
   constexpr bool BF16 = std::is_same<T, __nv_bfloat16>::value;
-  const int group = p.heads / p.kv_heads, tokens = BM / group;
   CUtensorMap mq, mk, mv, mo;
   // without keys k and v may be null: their maps are never used
-  const slim_view& k = p.kv_len > 0 ? p.k : p.q;
-  const slim_view& v = p.kv_len > 0 ? p.v : p.q;
-  if (!make_map(&mq, BF16, p.q, p.batch, p.q_len, p.heads, p.dim, group, tokens) ||
-      !make_map(&mo, BF16, p.out, p.batch, p.q_len, p.heads, p.dim, group, tokens) ||
-      !make_map(&mk, BF16, k, p.batch, p.kv_len > 0 ? p.kv_len : 1, p.kv_len > 0 ? p.kv_heads : 1, p.dim, 1, BN) ||
-      !make_map(&mv, BF16, v, p.batch, p.kv_len > 0 ? p.kv_len : 1, p.kv_len > 0 ? p.kv_heads : 1, p.dim, 1, BN))
+  const bool any = p.kv_len > 0;
+  if (!make_map(&mq, BF16, p.q, p.batch, p.q_len, p.heads, p.dim, plan.group, plan.tokens) ||
+      !make_map(&mo, BF16, p.out, p.batch, p.q_len, p.heads, p.dim, plan.group, plan.tokens) ||
+      !make_map(&mk, BF16, any ? p.k : p.q, p.batch, any ? p.kv_len : 1, any ? p.kv_heads : 1, p.dim, 1, BN) ||
+      !make_map(&mv, BF16, any ? p.v : p.q, p.batch, any ? p.kv_len : 1, any ? p.kv_heads : 1, p.dim, 1, BN))
     return cudaErrorInvalidValue;
   int dev = 0;
   cudaGetDevice(&dev);
   static PerDeviceOnce once;
-  const cudaError_t e = once.run(dev, [] {
-    return cudaFuncSetAttribute(tile_kernel<T, DP, MASK>, cudaFuncAttributeMaxDynamicSharedMemorySize,
-                                static_cast<int>(smem_bytes<DP>()));
+  constexpr size_t smem = smem_bytes<DP, SPLIT>();
+  cudaError_t e = once.run(dev, [] {
+    return cudaFuncSetAttribute(tile_kernel<T, DP, BIAS, SPLIT>, cudaFuncAttributeMaxDynamicSharedMemorySize,
+                                static_cast<int>(smem));
   });
   if (e != cudaSuccess) return e;
-  const TileParams tp{p.q_len, p.kv_len, group, tokens, p.k.stride_b != 0, p.k.stride_h != 0, p.v.stride_b != 0,
-                      p.v.stride_h != 0, p.scale2, p.bias, p.bias_pitch, p.n_keys};
-  const dim3 grid(static_cast<unsigned>((p.q_len + 2 * tokens - 1) / (2 * tokens)), static_cast<unsigned>(p.kv_heads),
-                  static_cast<unsigned>(p.batch));
-  tile_kernel<T, DP, MASK><<<grid, THREADS, smem_bytes<DP>(), st>>>(mq, mk, mv, mo, tp);
-  return cudaGetLastError();
+  const TileParams tp{p.q_len, p.kv_len, plan.group, plan.tokens, p.k.stride_b != 0, p.k.stride_h != 0,
+                      p.v.stride_b != 0, p.v.stride_h != 0, p.scale2, p.keys, plan.splits, plan.per, plan.rows, p.partial};
+  const int64_t x = SPLIT ? plan.q_tiles * plan.splits : (plan.q_tiles + 1) / 2;
+  const dim3 grid(static_cast<unsigned>(x), static_cast<unsigned>(p.kv_heads), static_cast<unsigned>(p.batch));
+  tile_kernel<T, DP, BIAS, SPLIT><<<grid, THREADS, smem, st>>>(mq, mk, mv, mo, tp);
+  if ((e = cudaGetLastError()) != cudaSuccess) return e;
+  note_launch();
+  if (SPLIT) {
+    const int64_t items = p.batch * p.kv_heads * plan.q_tiles;
+    split_kernel<T, DP><<<static_cast<unsigned>(items * plan.rows), 256, 0, st>>>(
+        p.partial, p.out, p.q_len, plan.group, plan.tokens, plan.rows, static_cast<int>(plan.q_tiles), p.kv_heads,
+        2 * plan.splits, items, p.dim);
+    if ((e = cudaGetLastError()) != cudaSuccess) return e;
+    note_launch();
+  }
+  return cudaSuccess;
 }
 
-template <typename T>
-cudaError_t launch(const Params& p, cudaStream_t st) {
-  if (p.bias != nullptr) return p.dim > 64 ? launch<T, 128, true>(p, st) : launch<T, 64, true>(p, st);
-  return p.dim > 64 ? launch<T, 128, false>(p, st) : launch<T, 64, false>(p, st);
+template <typename T, int DP>
+cudaError_t launch(const Params& p, const Plan& plan, cudaStream_t st) {
+  if (plan.splits > 0)
+    return p.keys.bias != nullptr ? launch<T, DP, true, true>(p, plan, st) : launch<T, DP, false, true>(p, plan, st);
+  return p.keys.bias != nullptr ? launch<T, DP, true, false>(p, plan, st) : launch<T, DP, false, false>(p, plan, st);
 }
 }  // namespace tile
 
 struct Workspace {
-  int64_t bias, n_keys, total, pitch;
+  int64_t bias, n_keys, partial, total, pitch;
 };
 
-static Workspace workspace(int64_t batch, int64_t kv_len, bool masked) {
+static Workspace workspace(int64_t batch, int64_t kv_len, bool additive, const tile::Plan& plan) {
+  auto up = [](int64_t v) { return (v + 255) / 256 * 256; };
   Workspace w{};
   w.pitch = (kv_len + KEY_TILE - 1) / KEY_TILE * KEY_TILE;
-  if (masked) {
-    w.bias = 0;
-    w.n_keys = (batch * w.pitch * 4 + 255) / 256 * 256;
-    w.total = w.n_keys + (batch * 4 + 255) / 256 * 256;
+  if (additive) {
+    w.n_keys = up(batch * w.pitch * 4);
+    w.total = w.n_keys + up(batch * 4);
   }
+  w.partial = w.total;
+  w.total += up(plan.floats * 4);
   return w;
 }
 
@@ -575,11 +761,12 @@ using namespace slim;
 extern "C" {
 
 int slim_cross_attn_workspace_bytes(int64_t batch, int64_t q_len, int64_t kv_len, int heads, int kv_heads, int dim,
-                                    int masked, uint64_t* bytes) {
+                                    int additive, uint64_t* bytes) {
   const int rc = xattn::checks(batch, q_len, kv_len, heads, kv_heads, dim);
   if (rc != SLIM_OK) return rc;
   if (bytes == nullptr) return fail(SLIM_ERR_NULL, "bytes is NULL");
-  *bytes = static_cast<uint64_t>(xattn::workspace(batch, kv_len, masked != 0).total);
+  const xattn::tile::Plan plan = xattn::tile::make_plan(batch, q_len, kv_len, heads, kv_heads, dim);
+  *bytes = static_cast<uint64_t>(xattn::workspace(batch, kv_len, additive != 0, plan).total);
   return SLIM_OK;
 }
 
@@ -603,8 +790,9 @@ int slim_cross_attn(const slim_view* q, const slim_view* k, const slim_view* v, 
   if (!xattn::view_ok(q, batch, q_len, heads, false) || !xattn::view_ok(out, batch, q_len, heads, false) ||
       (kv_len > 0 && (!xattn::view_ok(k, batch, kv_len, kv_heads, true) || !xattn::view_ok(v, batch, kv_len, kv_heads, true))))
     return fail(SLIM_ERR_ALIGN, "rows of q/k/v/out must be 16-byte aligned with positive strides (0 for shared k/v)");
-  const bool masked = kv_len > 0 && (mask != nullptr || kv_lengths != nullptr);
-  const xattn::Workspace w = xattn::workspace(batch, kv_len, masked);
+  const bool additive = kv_len > 0 && mask != nullptr && mask_type != SLIM_MASK_BOOL;
+  const xattn::tile::Plan plan = xattn::tile::make_plan(batch, q_len, kv_len, heads, kv_heads, dim);
+  const xattn::Workspace w = xattn::workspace(batch, kv_len, additive, plan);
   if (workspace_bytes < static_cast<uint64_t>(w.total))
     return fail(SLIM_ERR_SHAPE, "workspace of %llu bytes is smaller than the %lld needed",
                 static_cast<unsigned long long>(workspace_bytes), static_cast<long long>(w.total));
@@ -612,23 +800,33 @@ int slim_cross_attn(const slim_view* q, const slim_view* k, const slim_view* v, 
   if (!aligned16(ws)) return fail(SLIM_ERR_ALIGN, "workspace must be 16-byte aligned");
   if ((rc = check_arch()) != SLIM_OK) return rc;
   cudaStream_t st = static_cast<cudaStream_t>(stream);
-  xattn::Params p{*q, *k, *v, *out, batch, q_len, kv_len, heads, kv_heads, dim, scale * xattn::kLog2e, nullptr, 0, nullptr};
+  uint8_t* base = static_cast<uint8_t*>(ws);
+  xattn::Params p{*q, *k, *v, *out, batch, q_len, kv_len, heads, kv_heads, dim, scale * xattn::kLog2e, {}, nullptr};
+  if (plan.floats > 0) p.partial = reinterpret_cast<float*>(base + w.partial);
   cudaError_t e;
-  if (masked) {
-    float* bias = reinterpret_cast<float*>(static_cast<uint8_t*>(ws) + w.bias);
-    int* n_keys = reinterpret_cast<int*>(static_cast<uint8_t*>(ws) + w.n_keys);
-    xattn::bias_kernel<<<static_cast<unsigned>(batch), 1024, 0, st>>>(
-        mask, mask != nullptr ? mask_type : xattn::kMaskNone, mask_stride_b, mask_stride_k, kv_lengths,
-        lengths_bits == 64, kv_len, w.pitch, bias, n_keys);
+  if (additive) {
+    float* bias = reinterpret_cast<float*>(base + w.bias);
+    int* n_keys = reinterpret_cast<int*>(base + w.n_keys);
+    xattn::bias_kernel<<<static_cast<unsigned>(batch), 1024, 0, st>>>(mask, mask_type, mask_stride_b, mask_stride_k,
+                                                                      kv_lengths, lengths_bits == 64, kv_len, w.pitch,
+                                                                      bias, n_keys);
     if ((e = cudaGetLastError()) != cudaSuccess) return cuda_fail(e, "attention mask launch");
     note_launch();
-    p.bias = bias;
-    p.bias_pitch = w.pitch;
-    p.n_keys = n_keys;
+    p.keys.bias = bias;
+    p.keys.bias_pitch = w.pitch;
+    p.keys.n_keys = n_keys;
+  } else if (kv_len > 0) {
+    p.keys.mask = static_cast<const uint8_t*>(mask);
+    p.keys.mask_b = mask_stride_b;
+    p.keys.mask_k = mask_stride_k;
+    p.keys.lengths = kv_lengths;
+    p.keys.lengths64 = lengths_bits == 64;
   }
-  e = dtype == kBF16 ? xattn::tile::launch<__nv_bfloat16>(p, st) : xattn::tile::launch<__half>(p, st);
+  if (dtype == kBF16)
+    e = dim > 64 ? xattn::tile::launch<__nv_bfloat16, 128>(p, plan, st) : xattn::tile::launch<__nv_bfloat16, 64>(p, plan, st);
+  else
+    e = dim > 64 ? xattn::tile::launch<__half, 128>(p, plan, st) : xattn::tile::launch<__half, 64>(p, plan, st);
   if (e != cudaSuccess) return cuda_fail(e, "cross attention launch");
-  note_launch();
   return SLIM_OK;
 }
 

@@ -306,10 +306,10 @@ def cross_attention(q, k, v, key_mask=None, kv_lengths=None, scale: float | None
     scale = max(d, 1) ** -0.5 if scale is None else float(scale)
     lib = nat.load()
     out = torch.empty((b, sq, h, d), dtype=q4.dtype, device=dev)
-    masked = key_mask is not None or kv_lengths is not None
+    additive = key_mask is not None and key_mask.dtype != torch.bool
     need = ctypes.c_uint64(0)
     with torch.cuda.device(dev):
-        nat.check(lib.slim_cross_attn_workspace_bytes(b, sq, sk, h, hk, d, int(masked), ctypes.byref(need)))
+        nat.check(lib.slim_cross_attn_workspace_bytes(b, sq, sk, h, hk, d, int(additive), ctypes.byref(need)))
         ws = torch.empty((need.value,), dtype=torch.uint8, device=dev) if need.value else None
         nat.check(lib.slim_cross_attn(
             _view(q4), _view(k4), _view(v4), _view(out), nat.BF16 if q4.dtype == torch.bfloat16 else nat.F16, b, sq, sk,
