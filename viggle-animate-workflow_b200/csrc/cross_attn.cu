@@ -114,22 +114,28 @@ __global__ void __launch_bounds__(1024) bias_kernel(const void* __restrict__ mas
 //   wide   256 rows of one (sequence, key head), every key tile loaded once for both
 //   SPLIT  for few rows: one tile of rows, its keys cut over several CTAs and within a CTA over the
 //          two tiles (even and odd key tiles); partial sums go to memory and split_kernel joins them
-// 10 warps:
-//   warps 0..3, 4..7  softmax of tile 0 / 1, one row a thread: the scores are read from TMEM twice
-//                     (row maximum, then weights 2^(s scale2 + bias - m)), the weights go back packed
-//                     to 16 bits over the scores they came from, where the second product reads them.
+// 12 warps (the last idle):
+//   warps 0..3, 4..7  softmax of tile 0 / 1, one row a thread: row maximum, then weights
+//                     2^(s scale2 + bias - m), which go back packed to 16 bits over the scores they
+//                     came from, where the second product reads them (in two halves).
 //                     O is rescaled only when a maximum grows by more than 2^8 over the one in use
 //                     (the weights stay below 2^8, sums and O are fp32), which is rare after the
 //                     first tile.
 //   warp 8            TMA: the Q tiles, then key and value tiles in the order of their use, one ring
-//   warp 9            TMEM, and the MMAs: S_t = Q_t K_j^T, then per tile O_t += P_t V_j followed at
+//   warps 9, 10       the MMAs of tile 0 / 1: S_t = Q_t K_0^T, then per step O_t += P_t V_j followed at
 //                     once by S_t = Q_t K_{j+1}^T: while one tile is in the softmax the tensor cores
-//                     work on the other.
+//                     work on the other. One warp for both tiles left the tensor cores idle while it
+//                     waited and committed (about 650 cycles a tile and step): 2.74 -> XX ms at
+//                     16384 x 16111 x 24 heads of 128.
 // V is read as it lies (keys x head elements): an MN-major operand. Excluded keys have weight 0; their
 // rows of V are cleared in shared memory, as 0 * NaN is not 0.
 namespace tile {
 constexpr int BM = 128, BN = KEY_TILE;
-constexpr int WARPS = 10, THREADS = 32 * WARPS;
+constexpr int WARPS = 12, THREADS = 32 * WARPS;
+// Registers: 168 a thread at launch, of which the softmax warpgroups take 208 each (a row of 128 scores
+// stays in registers) and the third leaves all but 88: 2 x 208 + 88 = 3 x 168.
+constexpr int REGS = 168, REGS_SOFTMAX = 208, REGS_OTHER = 88;
+static_assert(2 * REGS_SOFTMAX + REGS_OTHER <= 3 * REGS, "the register shares exceed the launch's allocation");
 __device__ __forceinline__ constexpr uint32_t col_s(int t) { return t * 128u; }         // scores, then weights
 __device__ __forceinline__ constexpr uint32_t col_o(int t) { return 256u + t * 128u; }  // output accumulator
 constexpr float GROWTH = 8.0f;  // base-2 growth of a maximum that is let stand
@@ -149,8 +155,9 @@ template <int STAGES>
 struct Shared {
   uint64_t q_full[2];
   uint64_t full[STAGES], empty[STAGES];
-  uint64_t s_full[2], p_full[2], o_full[2];
-  uint64_t drain;
+  uint64_t s_full[2], p_full[2][2], o_full[2];  // p_full: the weights of the first / second half of the keys
+  uint64_t turn[2];   // wide: the tile whose MMAs may be issued
+  uint64_t drain[2];
   uint32_t tmem_base;
   volatile int abort;
 };
@@ -192,34 +199,15 @@ __device__ __forceinline__ uint32_t pack2<__half>(float lo, float hi) {
   return *reinterpret_cast<const uint32_t*>(&h);
 }
 
-// 32 scores of one row from TMEM: s where the bit is set and -inf elsewhere, or (BIAS) s scale2 + bias.
-template <bool BIAS>
-__device__ __forceinline__ void load_scores(uint32_t taddr, int c, const float4* bias4, float scale2, uint32_t bits,
-                                            float (&y)[32]) {
-  uint32_t r[32];
-  tmem_ld_32x32b_x32(taddr + c, r);
-  tmem_ld_wait();
-  reg_dep32(r);
+// Base-2 weights of 64 keys: w = 2^(y sc + off), summed in fp32, packed to the type of v.
+template <typename T>
+__device__ __forceinline__ void weights(const float* y, float2 sc2, float2 off2, float2& l2, uint32_t (&w)[32]) {
 #pragma unroll
-  for (int e = 0; e < 32; ++e) y[e] = __uint_as_float(r[e]);
-  if (BIAS) {
-    if (bits == 0) {  // behind the last key: the bias row may end here
-#pragma unroll
-      for (int e = 0; e < 32; ++e) y[e] = -INFINITY;
-      return;
-    }
-#pragma unroll
-    for (int e = 0; e < 32; e += 4) {
-      const float4 b = __ldg(bias4 + (c + e) / 4);
-      // an excluded key's score may be NaN
-      y[e + 0] = b.x == -INFINITY ? -INFINITY : fmaf(y[e + 0], scale2, b.x);
-      y[e + 1] = b.y == -INFINITY ? -INFINITY : fmaf(y[e + 1], scale2, b.y);
-      y[e + 2] = b.z == -INFINITY ? -INFINITY : fmaf(y[e + 2], scale2, b.z);
-      y[e + 3] = b.w == -INFINITY ? -INFINITY : fmaf(y[e + 3], scale2, b.w);
-    }
-  } else if (bits != 0xffffffffu) {
-#pragma unroll
-    for (int e = 0; e < 32; ++e) y[e] = (bits >> e) & 1 ? y[e] : -INFINITY;
+  for (int e = 0; e < 32; ++e) {
+    const float2 x = fma2(make_float2(y[2 * e], y[2 * e + 1]), sc2, off2);
+    const float2 g = make_float2(ex2_approx(x.x), ex2_approx(x.y));
+    l2 = add2(l2, g);
+    w[e] = pack2<T>(g.x, g.y);
   }
 }
 
@@ -262,14 +250,16 @@ tile_kernel(const __grid_constant__ CUtensorMap tq, const __grid_constant__ CUte
     for (int t = 0; t < 2; ++t) {
       mbar_init(&sh.q_full[t], 1);
       mbar_init(&sh.s_full[t], 1);
-      mbar_init(&sh.p_full[t], BM);
+      mbar_init(&sh.p_full[t][0], BM / 32);
+      mbar_init(&sh.p_full[t][1], BM / 32);
       mbar_init(&sh.o_full[t], 1);
+      mbar_init(&sh.turn[t], 1);
+      mbar_init(&sh.drain[t], 1);
     }
     for (int s = 0; s < L::STAGES; ++s) {
       mbar_init(&sh.full[s], 1);
-      mbar_init(&sh.empty[s], 1);
+      mbar_init(&sh.empty[s], SPLIT ? 1 : tiles);  // wide: both tiles have used it
     }
-    mbar_init(&sh.drain, 1);
     sh.abort = 0;
     fence_mbar_init();
   }
@@ -282,6 +272,8 @@ tile_kernel(const __grid_constant__ CUtensorMap tq, const __grid_constant__ CUte
   tc_fence_after();
   const uint32_t tmem = sh.tmem_base;
 
+  if (warp >= 8) {
+    regs_dec<REGS_OTHER>();
   if (warp == 8) {
     // ------------------------------------------------------------ TMA producer
     if (lane == 0 && steps > 0) {
@@ -316,58 +308,86 @@ tile_kernel(const __grid_constant__ CUtensorMap tq, const __grid_constant__ CUte
       for (int s = 0; s < L::STAGES; ++s)
         if (issued & (1u << s)) mbar_wait(&sh.full[s], (last_parity >> s) & 1, kErrWaitTimeoutDrain);
     }
-  } else if (warp == 9) {
-    // ------------------------------------------------------------ MMA issue
+  } else if (warp - 9 < tiles) {
+    // ------------------------------------------------------------ MMA issue of tile t
+    const int t = warp - 9;
     if (lane == 0 && steps > 0) {
-      bool ok = true;
-      auto wait = [&](uint64_t* bar, uint32_t parity) {
-        ok = ok && mbar_wait(bar, parity, kErrWaitTimeoutMma) && !sh.abort;
-        return ok;
+      auto wait = [&](uint64_t* bar, uint32_t parity) { return mbar_wait_abort(bar, parity, kErrWaitTimeoutMma, &sh.abort); };
+      // the ring position of load i, carried along as (slot, parity) instead of dividing
+      struct Ring {
+        int slot, parity;
+        __device__ __forceinline__ Ring at(int n) const {
+          const int s = slot + n;
+          return s >= L::STAGES ? Ring{s - L::STAGES, parity ^ 1} : Ring{s, parity};
+        }
       };
-      auto full = [&](int i) { return wait(&sh.full[i % L::STAGES], (i / L::STAGES) & 1); };
-      auto qk = [&](int t, int i) {
-        const uint32_t qa = smem_u32(sQ + (SPLIT ? 0 : t * L::TILE_BYTES));
-        const uint32_t ka = smem_u32(sKV + (i % L::STAGES) * L::TILE_BYTES);
+      auto full = [&](Ring r) { return wait(&sh.full[r.slot], r.parity); };
+      const uint64_t q_desc = smem_desc_sw128(smem_u32(sQ + (SPLIT ? 0 : t * L::TILE_BYTES)));
+      const uint32_t kv_addr = smem_u32(sKV);
+      const uint32_t t_s = tmem + col_s(t), t_o = tmem + col_o(t);
+      auto qk = [&](Ring r) {
+        const uint64_t kd = smem_desc_sw128(kv_addr + r.slot * L::TILE_BYTES);
 #pragma unroll
         for (int k = 0; k < DP / 16; ++k) {
           const uint32_t off = (k >> 2) * L::BLOCK_BYTES + (k & 3) * 32;
-          mma_f16(tmem + col_s(t), smem_desc_sw128(qa + off), smem_desc_sw128(ka + off), IDESC_QK, k != 0);
+          mma_f16(t_s, smem_desc_at(q_desc, off), smem_desc_at(kd, off), IDESC_QK, k != 0);
         }
         mma_commit(&sh.s_full[t]);
-        if (SPLIT || t == tiles - 1) mma_commit(&sh.empty[i % L::STAGES]);
+        mma_commit(&sh.empty[r.slot]);
       };
-      auto pv = [&](int t, int i, bool first) {
-        const uint32_t va = smem_u32(sKV + (i % L::STAGES) * L::TILE_BYTES);
-#pragma unroll
-        for (int k = 0; k < BN / 16; ++k)
-          mma_f16_ta(tmem + col_o(t), tmem + col_s(t) + k * 8, smem_desc_mn_sw128(va + k * 2048, L::BLOCK_BYTES),
-                     IDESC_PV, !(first && k == 0));
-        mma_commit(&sh.o_full[t]);
-        if (SPLIT || t == tiles - 1) mma_commit(&sh.empty[i % L::STAGES]);
+      // Both tiles' MMAs share the tensor cores. Issued as they come they interleave, both tiles finish
+      // late and their softmaxes run in step; so each batch (second product, next scores) is issued as
+      // a whole and the tiles take turns.
+      auto my_turn = [&](int k) { return tiles == 1 || wait(&sh.turn[t], t == 0 ? (k & 1) ^ 1 : k & 1); };
+      auto pass_turn = [&] {
+        if (tiles == 2) mbar_arrive(&sh.turn[t ^ 1]);
       };
-      for (int t = 0; t < tiles; ++t) {
-        if (!full(k_load(t, 0)) || !wait(&sh.q_full[SPLIT ? 0 : t], 0)) break;
+      auto pv = [&](Ring r, int j) {
+        const uint64_t vd = smem_desc_mn_sw128(kv_addr + r.slot * L::TILE_BYTES, L::BLOCK_BYTES);
+#ifdef HALFHOLD
+        if (!wait(&sh.p_full[t][0], j & 1) || !my_turn(j + 1)) return false;
+#else
+        if (!wait(&sh.p_full[t][0], j & 1) || !wait(&sh.p_full[t][1], j & 1) || !my_turn(j + 1)) return false;
+#endif
         tc_fence_after();
-        qk(t, k_load(t, 0));
+#pragma unroll
+        for (int k = 0; k < BN / 16; ++k) {
+#ifdef HALFHOLD
+          if (k == BN / 32) {
+            if (!wait(&sh.p_full[t][1], j & 1)) return false;
+            tc_fence_after();
+          }
+#endif
+          mma_f16_ta(t_o, t_s + k * 8, smem_desc_at(vd, k * 2048), IDESC_PV, j != 0 || k != 0);
+        }
+        mma_commit(&sh.o_full[t]);
+        mma_commit(&sh.empty[r.slot]);
+        return true;
+      };
+      Ring base{0, 0};  // of the step's first load
+      bool ok = full(base.at(k_load(t, 0))) && wait(&sh.q_full[SPLIT ? 0 : t], 0) && my_turn(0);
+      if (ok) {
+        tc_fence_after();
+        qk(base.at(k_load(t, 0)));
+        pass_turn();
       }
       for (int j = 0; ok && j < steps; ++j) {
-        for (int t = 0; t < tiles; ++t) {
-          if (!full(v_load(t, j)) || !wait(&sh.p_full[t], j & 1)) break;
-          tc_fence_after();
-          pv(t, v_load(t, j), j == 0);
-          if (j + 1 < steps) {
-            if (!full(k_load(t, j + 1))) break;
-            tc_fence_after();
-            qk(t, k_load(t, j + 1));
-          }
-        }
+        const Ring next = base.at(SPLIT ? 4 : 2);
+        const bool more = j + 1 < steps;
+        ok = full(base.at(v_load(t, 0))) && (!more || full(next.at(k_load(t, 0)))) && pv(base.at(v_load(t, 0)), j);
+        if (ok && more) qk(next.at(k_load(t, 0)));
+        pass_turn();
+        base = next;
       }
       if (!ok) sh.abort = 1;
-      mma_commit(&sh.drain);
-      mbar_wait(&sh.drain, 0, kErrWaitTimeoutDrain);
+      mma_commit(&sh.drain[t]);
+      mbar_wait(&sh.drain[t], 0, kErrWaitTimeoutDrain);
     }
     __syncwarp();
-  } else if ((warp >> 2) < tiles) {
+  }
+  } else {
+    regs_inc<REGS_SOFTMAX>();
+    if ((warp >> 2) < tiles) {
     // ------------------------------------------------------------ softmax of one row, output
     const int t = warp >> 2;
     const int quarter = warp & 3;
@@ -377,11 +397,10 @@ tile_kernel(const __grid_constant__ CUtensorMap tq, const __grid_constant__ CUte
     const float scale2 = p.scale2;
     // few rows: warps whose rows do not exist only keep step
     const bool live = !SPLIT || quarter * 32 < p.rows;
+    // 128 rows need not be a whole number of tokens: what is left in the others has no say in rescaling
+    const bool real = row < p.group * p.tokens;
     auto wait = [&](uint64_t* bar, uint32_t parity) {
-      bool ok = mbar_wait(bar, parity, kErrWaitTimeoutEpilogue);
-      ok = __all_sync(0xffffffffu, ok) && !sh.abort;
-      if (!ok) sh.abort = 1;
-      return ok;
+      return __all_sync(0xffffffffu, mbar_wait_abort(bar, parity, kErrWaitTimeoutEpilogue, &sh.abort)) != 0;
     };
     bool good = true;
     float m = -INFINITY;
@@ -405,7 +424,7 @@ tile_kernel(const __grid_constant__ CUtensorMap tq, const __grid_constant__ CUte
           bits[w] = __ballot_sync(0xffffffffu, in);
         }
       }
-      if (SPLIT || t == 0) {  // wide: tile 0's weights gate the second product of both tiles
+      {  // wide: both tiles clear the same rows, each before its own second product
         const uint32_t mine = quarter == 0 ? bits[0] : quarter == 1 ? bits[1] : quarter == 2 ? bits[2] : bits[3];
         bool clear = !((mine >> lane) & 1) && key0 + row < p.kv_len;
         if (BIAS && !clear) clear = row < left && __ldg(reinterpret_cast<const float*>(bias4) + row) == -INFINITY;
@@ -425,25 +444,41 @@ tile_kernel(const __grid_constant__ CUtensorMap tq, const __grid_constant__ CUte
       if (!(good = wait(&sh.s_full[t], j & 1))) break;
       tc_fence_after();
       if (live) {
-        float top = -INFINITY;
+        uint32_t r[BN];
 #pragma unroll
-        for (int c = 0; c < BN; c += 32) {
-          float y[32];
-          load_scores<BIAS>(t_s, c, bias4, scale2, bits[c / 32], y);
-          float mx[4] = {y[0], y[1], y[2], y[3]};
+        for (int c = 0; c < BN; c += 32) tmem_ld_32x32b_x32(t_s + c, *reinterpret_cast<uint32_t(*)[32]>(r + c));
+        tmem_ld_wait();
 #pragma unroll
-          for (int e = 4; e < 28; e += 8) {
+        for (int c = 0; c < BN; c += 32) reg_dep32(*reinterpret_cast<uint32_t(*)[32]>(r + c));
+        float* y = reinterpret_cast<float*>(r);
+        if (BIAS) {
 #pragma unroll
-            for (int u = 0; u < 4; ++u) mx[u] = fmax3(mx[u], y[e + u], y[e + 4 + u]);
+          for (int e = 0; e < BN; e += 4) {
+            // an excluded key's score may be NaN; behind the last key the bias row may have ended
+            const float4 a = (bits[e / 32] >> (e & 31)) & 1 ? __ldg(bias4 + e / 4)
+                                                            : make_float4(-INFINITY, -INFINITY, -INFINITY, -INFINITY);
+            y[e + 0] = a.x == -INFINITY ? -INFINITY : fmaf(y[e + 0], scale2, a.x);
+            y[e + 1] = a.y == -INFINITY ? -INFINITY : fmaf(y[e + 1], scale2, a.y);
+            y[e + 2] = a.z == -INFINITY ? -INFINITY : fmaf(y[e + 2], scale2, a.z);
+            y[e + 3] = a.w == -INFINITY ? -INFINITY : fmaf(y[e + 3], scale2, a.w);
           }
+        } else if ((bits[0] & bits[1] & bits[2] & bits[3]) != 0xffffffffu) {
 #pragma unroll
-          for (int u = 0; u < 4; ++u) mx[u] = fmaxf(mx[u], y[28 + u]);
-          top = fmaxf(top, fmaxf(fmax3(mx[0], mx[1], mx[2]), mx[3]));
+          for (int e = 0; e < BN; ++e) y[e] = (bits[e / 32] >> (e & 31)) & 1 ? y[e] : -INFINITY;
         }
+        float mx[4] = {y[0], y[1], y[2], y[3]};
+#pragma unroll
+        for (int e = 4; e < BN - 4; e += 8) {
+#pragma unroll
+          for (int u = 0; u < 4; ++u) mx[u] = fmax3(mx[u], y[e + u], y[e + 4 + u]);
+        }
+#pragma unroll
+        for (int u = 0; u < 4; ++u) mx[u] = fmaxf(mx[u], y[BN - 4 + u]);
+        const float top = fmaxf(fmax3(mx[0], mx[1], mx[2]), mx[3]);
         const float m_new = fmaxf(m, BIAS ? top : top * scale2);
         if (j == 0) {
           m = m_new;
-        } else if (__any_sync(0xffffffffu, m_new > m + GROWTH)) {
+        } else if (__any_sync(0xffffffffu, real && m_new > m + GROWTH)) {
           const float alpha = m_new == -INFINITY ? 1.0f : ex2_approx(m - m_new);
           m = m_new;
           l2 = mul2(l2, make_float2(alpha, alpha));
@@ -461,26 +496,22 @@ tile_kernel(const __grid_constant__ CUtensorMap tq, const __grid_constant__ CUte
           }
         }
         const float off = m == -INFINITY ? 0.0f : -m;
-        const float2 off2 = make_float2(off, off), sc2 = make_float2(scale2, scale2);
+        const float sc = BIAS ? 1.0f : scale2;
+        const float2 off2 = make_float2(off, off), sc2 = make_float2(sc, sc);
 #pragma unroll
-        for (int c = 0; c < BN; c += 32) {
-          float y[32];
-          load_scores<BIAS>(t_s, c, bias4, scale2, bits[c / 32], y);
-          uint32_t w[16];
-#pragma unroll
-          for (int e = 0; e < 16; ++e) {
-            const float2 a = make_float2(y[2 * e], y[2 * e + 1]);
-            const float2 x = BIAS ? add2(a, off2) : fma2(a, sc2, off2);
-            const float2 g = make_float2(ex2_approx(x.x), ex2_approx(x.y));
-            l2 = add2(l2, g);
-            w[e] = pack2<T>(g.x, g.y);
-          }
-          tmem_st_32x32b_x16(t_s + c / 2, w);
+        for (int half = 0; half < 2; ++half) {
+          uint32_t w[32];
+          weights<T>(y + 64 * half, sc2, off2, l2, w);
+          tmem_st_32x32b_x32(t_s + 32 * half, w);
+          tmem_st_wait();
+          tc_fence_before();
+          __syncwarp();
+          if (lane == 0) mbar_arrive(&sh.p_full[t][half]);
         }
-        tmem_st_wait();
+      } else {
+        __syncwarp();
+        if (lane < 2) mbar_arrive(&sh.p_full[t][lane]);
       }
-      tc_fence_before();
-      mbar_arrive(&sh.p_full[t]);
     }
     const float l = l2.x + l2.y;
     if (good && steps > 0) {
@@ -549,6 +580,7 @@ tile_kernel(const __grid_constant__ CUtensorMap tq, const __grid_constant__ CUte
         bulk_wait_group<0>();
       }
     }
+    }
   }
   tc_fence_before();
   __syncthreads();
@@ -567,7 +599,7 @@ __global__ void __launch_bounds__(256) split_kernel(const float* __restrict__ pa
                                                     int parts, int64_t items, int dim) {
   constexpr int E = DP / 32;
   __shared__ float s_o[8][DP];
-  __shared__ float s_l[8], s_m[8];
+  __shared__ float s_l[8];
   const int lane = threadIdx.x & 31, warp = threadIdx.x >> 5;
   const int64_t item = blockIdx.x / rows;
   const int row = static_cast<int>(blockIdx.x - item * rows);
@@ -640,9 +672,10 @@ struct Plan {
   int64_t floats;             // of partial results
 };
 
-// The wide form takes 2 row tiles x key tiles steps per CTA; SPLIT 1 row tile x 2 key tiles a step, more
-// CTAs, and a second launch. Costs in steps (about 2.5 us): a wave of CTAs has to start and end (2), the
-// join costs 1.5. The cheapest wins: with few rows SPLIT, with many waves of CTAs the wide form.
+// The wide form takes 2 row tiles x 1 key tile a step, SPLIT 1 row tile x 2 key tiles, which moves twice
+// the keys and values through L2 for the same work (a step takes 1.35 times as long at 16384 x 16111 x
+// 24 heads of 128). Costs in wide steps (about 2.2 us): a wave of CTAs has to start and end (2), joining
+// costs 1.5. The cheapest wins: few rows are split, many waves of CTAs are not.
 inline Plan make_plan(int64_t batch, int64_t q_len, int64_t kv_len, int heads, int kv_heads, int dim) {
   Plan p{};
   p.group = heads / kv_heads;
@@ -654,7 +687,7 @@ inline Plan make_plan(int64_t batch, int64_t q_len, int64_t kv_len, int heads, i
   for (int64_t s = 1; s <= 64 && 2 * (s - 1) < nk; ++s) {
     const int64_t per = (nk + 2 * s - 1) / (2 * s) * 2;
     if ((s - 1) * per >= nk) continue;  // the last CTAs would have nothing
-    const double cost = static_cast<double>(waves(base * p.q_tiles * s)) * (2.0 + static_cast<double>(per) / 2) + 1.5;
+    const double cost = static_cast<double>(waves(base * p.q_tiles * s)) * (2.0 + 1.35 * static_cast<double>(per) / 2) + 1.5;
     if (cost < best && base * p.q_tiles * s < (int64_t{1} << 24)) {
       best = cost;
       p.splits = static_cast<int>(s);
@@ -684,6 +717,10 @@ cudaError_t launch(const Params& p, const Plan& plan, cudaStream_t st) {
   static PerDeviceOnce once;
   constexpr size_t smem = smem_bytes<DP, SPLIT>();
   cudaError_t e = once.run(dev, [] {
+    cudaFuncAttributes attr;
+    cudaError_t err = cudaFuncGetAttributes(&attr, tile_kernel<T, DP, BIAS, SPLIT>);
+    if (err == cudaSuccess && attr.numRegs < REGS) err = cudaErrorInvalidConfiguration;  // the shares would not fit
+    if (err != cudaSuccess) return err;
     return cudaFuncSetAttribute(tile_kernel<T, DP, BIAS, SPLIT>, cudaFuncAttributeMaxDynamicSharedMemorySize,
                                 static_cast<int>(smem));
   });

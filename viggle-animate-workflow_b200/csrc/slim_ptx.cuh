@@ -94,6 +94,21 @@ __device__ __forceinline__ bool mbar_wait(uint64_t* bar, uint32_t parity, unsign
   }
 }
 
+// The same, giving up as well (without a code of its own) once another warp has set *abort.
+__device__ __forceinline__ bool mbar_wait_abort(uint64_t* bar, uint32_t parity, unsigned int code, volatile int* abort) {
+  if (mbar_try_wait(bar, parity)) return true;
+  const uint64_t t0 = global_ns();
+  while (true) {
+    if (mbar_try_wait(bar, parity)) return true;
+    if (*abort) return false;
+    if (global_ns() - t0 > SLIM_WAIT_LIMIT_NS) {
+      record_error(code);
+      *abort = 1;
+      return false;
+    }
+  }
+}
+
 // ---------------------------------------------------------------- TMA (no multicast)
 __device__ __forceinline__ void tma_prefetch_desc(const void* desc) {
   asm volatile("prefetch.tensormap [%0];" ::"l"(desc) : "memory");
@@ -437,6 +452,9 @@ __device__ __forceinline__ uint64_t smem_desc_mn_sw128(uint32_t saddr, uint32_t 
   return d;
 }
 
+// A descriptor whose start address lies `bytes` (a multiple of 16) further within its tile.
+__device__ __forceinline__ uint64_t smem_desc_at(uint64_t desc, uint32_t bytes) { return desc + (bytes >> 4); }
+
 // 4-D tiled loads and stores (see tma_load_2d / tma_store_2d), innermost coordinate first.
 __device__ __forceinline__ void tma_load_4d(void* smem_dst, const void* desc, uint64_t* bar, int32_t c0, int32_t c1,
                                             int32_t c2, int32_t c3) {
@@ -452,6 +470,17 @@ __device__ __forceinline__ void tma_store_4d(const void* desc, const void* smem_
       "cp.async.bulk.tensor.4d.global.shared::cta.bulk_group [%0, {%2, %3, %4, %5}], [%1];" ::"l"(desc),
       "r"(smem_u32(smem_src)), "r"(c0), "r"(c1), "r"(c2), "r"(c3)
       : "memory");
+}
+
+// Registers a thread of this warpgroup keeps (all four warps take part). inc waits until the block's
+// launch allocation has them, so the shares of all warpgroups must fit in it.
+template <int N>
+__device__ __forceinline__ void regs_inc() {
+  asm volatile("setmaxnreg.inc.sync.aligned.u32 %0;" ::"n"(N));
+}
+template <int N>
+__device__ __forceinline__ void regs_dec() {
+  asm volatile("setmaxnreg.dec.sync.aligned.u32 %0;" ::"n"(N));
 }
 
 // Barrier `id` (1..15) among `threads` threads of the CTA, whole warps.
