@@ -114,28 +114,28 @@ __global__ void __launch_bounds__(1024) bias_kernel(const void* __restrict__ mas
 //   wide   256 rows of one (sequence, key head), every key tile loaded once for both
 //   SPLIT  for few rows: one tile of rows, its keys cut over several CTAs and within a CTA over the
 //          two tiles (even and odd key tiles); partial sums go to memory and split_kernel joins them
-// 12 warps (the last idle):
-//   warps 0..3, 4..7  softmax of tile 0 / 1, one row a thread: row maximum, then weights
-//                     2^(s scale2 + bias - m), which go back packed to 16 bits over the scores they
-//                     came from, where the second product reads them (in two halves).
-//                     O is rescaled only when a maximum grows by more than 2^8 over the one in use
-//                     (the weights stay below 2^8, sums and O are fp32), which is rare after the
-//                     first tile.
-//   warp 8            TMA: the Q tiles, then key and value tiles in the order of their use, one ring
-//   warps 9, 10       the MMAs of tile 0 / 1: S_t = Q_t K_0^T, then per step O_t += P_t V_j followed at
+// 20 warps (the last idle):
+//   warps 0..7, 8..15  softmax of tile 0 / 1, half a row (64 keys) a thread: the scores come from TMEM, the
+//                     row maximum of both halves through shared memory, the weights 2^(s scale2 + bias
+//                     - m) go back packed to 16 bits over the scores, where the second product reads
+//                     them. O is rescaled only when a maximum grows by more than 2^8 over the one in use
+//                     (the weights stay below 2^8, sums and O are fp32), which is rare after the first
+//                     tile. With a whole row a thread one warp per scheduler worked on a tile, issued
+//                     its exponentials at half the unit's rate, and a step took XX cycles instead of XX.
+//   warp 16           TMA: the Q tiles, then key and value tiles in the order of their use, one ring
+//   warps 17, 18      the MMAs of tile 0 / 1: S_t = Q_t K_0^T, then per step O_t += P_t V_j followed at
 //                     once by S_t = Q_t K_{j+1}^T: while one tile is in the softmax the tensor cores
-//                     work on the other. One warp for both tiles left the tensor cores idle while it
-//                     waited and committed (about 650 cycles a tile and step): 2.74 -> XX ms at
-//                     16384 x 16111 x 24 heads of 128.
+//                     work on the other.
 // V is read as it lies (keys x head elements): an MN-major operand. Excluded keys have weight 0; their
 // rows of V are cleared in shared memory, as 0 * NaN is not 0.
 namespace tile {
 constexpr int BM = 128, BN = KEY_TILE;
-constexpr int WARPS = 12, THREADS = 32 * WARPS;
-// Registers: 168 a thread at launch, of which the softmax warpgroups take 208 each (a row of 128 scores
-// stays in registers) and the third leaves all but 88: 2 x 208 + 88 = 3 x 168.
-constexpr int REGS = 168, REGS_SOFTMAX = 208, REGS_OTHER = 88;
-static_assert(2 * REGS_SOFTMAX + REGS_OTHER <= 3 * REGS, "the register shares exceed the launch's allocation");
+constexpr int SOFTMAX_WARPS = 16, WARP_TMA = 16, WARP_MMA = 17;
+constexpr int WARPS = 20, THREADS = 32 * WARPS;
+// Registers: 96 a thread at launch, of which the softmax warps take 104 and the last warpgroup leaves
+// all but 64: 4 x 104 + 64 = 5 x 96.
+constexpr int REGS = 96, REGS_SOFTMAX = 104, REGS_OTHER = 64;
+static_assert(4 * REGS_SOFTMAX + REGS_OTHER <= 5 * REGS, "the register shares exceed the launch's allocation");
 __device__ __forceinline__ constexpr uint32_t col_s(int t) { return t * 128u; }         // scores, then weights
 __device__ __forceinline__ constexpr uint32_t col_o(int t) { return 256u + t * 128u; }  // output accumulator
 constexpr float GROWTH = 8.0f;  // base-2 growth of a maximum that is let stand
@@ -155,16 +155,18 @@ template <int STAGES>
 struct Shared {
   uint64_t q_full[2];
   uint64_t full[STAGES], empty[STAGES];
-  uint64_t s_full[2], p_full[2][2], o_full[2];  // p_full: the weights of the first / second half of the keys
+  uint64_t s_full[2], p_full[2], o_full[2];
   uint64_t turn[2];   // wide: the tile whose MMAs may be issued
   uint64_t drain[2];
   uint32_t tmem_base;
   volatile int abort;
+  float x[2][2][BM];  // a row's maxima over both halves of the keys: [tile][half][row]
 };
 
 template <int DP, bool SPLIT>
 constexpr size_t smem_bytes() {
-  return 1024 + Layout<DP, SPLIT>::OFF_SH + sizeof(Shared<Layout<DP, SPLIT>::STAGES>);
+  static_assert(Layout<DP, SPLIT>::OFF_SH + sizeof(Shared<Layout<DP, SPLIT>::STAGES>) <= 232448, "shared memory");
+  return Layout<DP, SPLIT>::OFF_SH + sizeof(Shared<Layout<DP, SPLIT>::STAGES>);
 }
 
 struct TileParams {
@@ -199,11 +201,11 @@ __device__ __forceinline__ uint32_t pack2<__half>(float lo, float hi) {
   return *reinterpret_cast<const uint32_t*>(&h);
 }
 
-// Base-2 weights of 64 keys: w = 2^(y sc + off), summed in fp32, packed to the type of v.
+// Base-2 weights of 32 keys: w = 2^(y sc + off), summed in fp32, packed to the type of v.
 template <typename T>
-__device__ __forceinline__ void weights(const float* y, float2 sc2, float2 off2, float2& l2, uint32_t (&w)[32]) {
+__device__ __forceinline__ void weights(const float* y, float2 sc2, float2 off2, float2& l2, uint32_t (&w)[16]) {
 #pragma unroll
-  for (int e = 0; e < 32; ++e) {
+  for (int e = 0; e < 16; ++e) {
     const float2 x = fma2(make_float2(y[2 * e], y[2 * e + 1]), sc2, off2);
     const float2 g = make_float2(ex2_approx(x.x), ex2_approx(x.y));
     l2 = add2(l2, g);
@@ -220,9 +222,12 @@ tile_kernel(const __grid_constant__ CUtensorMap tq, const __grid_constant__ CUte
   constexpr bool BF16 = std::is_same<T, __nv_bfloat16>::value;
   constexpr uint32_t IDESC_QK = idesc_f16(BM, BN, BF16, false);
   constexpr uint32_t IDESC_PV = idesc_f16(BM, DP, BF16, true);
-  extern __shared__ uint8_t smem_raw[];
-  const uint32_t raw_addr = smem_u32(smem_raw);
-  uint8_t* smem = smem_raw + (((raw_addr + 1023) & ~1023u) - raw_addr);
+  extern __shared__ __align__(1024) uint8_t tile_smem[];
+  uint8_t* smem = tile_smem;
+  if (smem_u32(smem) & 1023) {  // the swizzled tiles need it; there is no room to round up
+    record_error(kErrSmemAlign);
+    return;
+  }
   uint8_t* sQ = smem;
   uint8_t* sKV = smem + L::OFF_KV;
   Sh& sh = *reinterpret_cast<Sh*>(smem + L::OFF_SH);
@@ -250,8 +255,7 @@ tile_kernel(const __grid_constant__ CUtensorMap tq, const __grid_constant__ CUte
     for (int t = 0; t < 2; ++t) {
       mbar_init(&sh.q_full[t], 1);
       mbar_init(&sh.s_full[t], 1);
-      mbar_init(&sh.p_full[t][0], BM / 32);
-      mbar_init(&sh.p_full[t][1], BM / 32);
+      mbar_init(&sh.p_full[t], 2 * BM / 32);
       mbar_init(&sh.o_full[t], 1);
       mbar_init(&sh.turn[t], 1);
       mbar_init(&sh.drain[t], 1);
@@ -263,7 +267,7 @@ tile_kernel(const __grid_constant__ CUtensorMap tq, const __grid_constant__ CUte
     sh.abort = 0;
     fence_mbar_init();
   }
-  if (warp == 9) {
+  if (warp == WARP_MMA) {
     tmem_alloc(&sh.tmem_base, 512);
     tmem_relinquish();
   }
@@ -272,9 +276,9 @@ tile_kernel(const __grid_constant__ CUtensorMap tq, const __grid_constant__ CUte
   tc_fence_after();
   const uint32_t tmem = sh.tmem_base;
 
-  if (warp >= 8) {
+  if (warp >= SOFTMAX_WARPS) {
     regs_dec<REGS_OTHER>();
-  if (warp == 8) {
+  if (warp == WARP_TMA) {
     // ------------------------------------------------------------ TMA producer
     if (lane == 0 && steps > 0) {
       const uint32_t q_bytes = static_cast<uint32_t>(L::BLOCKS * 128 * p.group * p.tokens);
@@ -308,9 +312,9 @@ tile_kernel(const __grid_constant__ CUtensorMap tq, const __grid_constant__ CUte
       for (int s = 0; s < L::STAGES; ++s)
         if (issued & (1u << s)) mbar_wait(&sh.full[s], (last_parity >> s) & 1, kErrWaitTimeoutDrain);
     }
-  } else if (warp - 9 < tiles) {
+  } else if (warp - WARP_MMA < tiles) {
     // ------------------------------------------------------------ MMA issue of tile t
-    const int t = warp - 9;
+    const int t = warp - WARP_MMA;
     if (lane == 0 && steps > 0) {
       auto wait = [&](uint64_t* bar, uint32_t parity) { return mbar_wait_abort(bar, parity, kErrWaitTimeoutMma, &sh.abort); };
       // the ring position of load i, carried along as (slot, parity) instead of dividing
@@ -344,22 +348,11 @@ tile_kernel(const __grid_constant__ CUtensorMap tq, const __grid_constant__ CUte
       };
       auto pv = [&](Ring r, int j) {
         const uint64_t vd = smem_desc_mn_sw128(kv_addr + r.slot * L::TILE_BYTES, L::BLOCK_BYTES);
-#ifdef HALFHOLD
-        if (!wait(&sh.p_full[t][0], j & 1) || !my_turn(j + 1)) return false;
-#else
-        if (!wait(&sh.p_full[t][0], j & 1) || !wait(&sh.p_full[t][1], j & 1) || !my_turn(j + 1)) return false;
-#endif
+        if (!my_turn(j + 1) || !wait(&sh.p_full[t], j & 1)) return false;
         tc_fence_after();
 #pragma unroll
-        for (int k = 0; k < BN / 16; ++k) {
-#ifdef HALFHOLD
-          if (k == BN / 32) {
-            if (!wait(&sh.p_full[t][1], j & 1)) return false;
-            tc_fence_after();
-          }
-#endif
+        for (int k = 0; k < BN / 16; ++k)
           mma_f16_ta(t_o, t_s + k * 8, smem_desc_at(vd, k * 2048), IDESC_PV, j != 0 || k != 0);
-        }
         mma_commit(&sh.o_full[t]);
         mma_commit(&sh.empty[r.slot]);
         return true;
@@ -387,73 +380,79 @@ tile_kernel(const __grid_constant__ CUtensorMap tq, const __grid_constant__ CUte
   }
   } else {
     regs_inc<REGS_SOFTMAX>();
-    if ((warp >> 2) < tiles) {
-    // ------------------------------------------------------------ softmax of one row, output
-    const int t = warp >> 2;
+    if ((warp >> 3) < tiles) {
+    // ------------------------------------------------------------ softmax of half a row, output
+    const int t = warp >> 3;
+    const int half = (warp >> 2) & 1;  // of the keys of a tile, of the columns of O
     const int quarter = warp & 3;
     const int row = quarter * 32 + lane;
     const uint32_t t_lane = tmem + (static_cast<uint32_t>(quarter * 32) << 16);
-    const uint32_t t_s = t_lane + col_s(t), t_o = t_lane + col_o(t);
+    const uint32_t t_s = t_lane + col_s(t), t_o = t_lane + col_o(t) + half * (DP / 2);
     const float scale2 = p.scale2;
     // few rows: warps whose rows do not exist only keep step
     const bool live = !SPLIT || quarter * 32 < p.rows;
     // 128 rows need not be a whole number of tokens: what is left in the others has no say in rescaling
     const bool real = row < p.group * p.tokens;
-    auto wait = [&](uint64_t* bar, uint32_t parity) {
-      return __all_sync(0xffffffffu, mbar_wait_abort(bar, parity, kErrWaitTimeoutEpilogue, &sh.abort)) != 0;
-    };
+    // After a wait that failed the warp goes through its steps without work (every further wait fails at
+    // once), so that both halves meet at each of their barriers.
     bool good = true;
+    auto wait = [&](uint64_t* bar, uint32_t parity) {
+      good = __all_sync(0xffffffffu, mbar_wait_abort(bar, parity, kErrWaitTimeoutEpilogue, &sh.abort)) != 0 && good;
+    };
     float m = -INFINITY;
     float2 l2 = make_float2(0.0f, 0.0f);
     for (int j = 0; j < steps; ++j) {
       const int64_t key0 = static_cast<int64_t>(key_tile(t, j)) * BN;
-      const float4* bias4 = BIAS ? reinterpret_cast<const float4*>(p.keys.bias + b * p.keys.bias_pitch + key0) : nullptr;
-      // one bit per key of the tile that takes part (with a bias: per key up to the last one)
-      const int64_t left = keys - key0;
-      uint32_t bits[4];
+      const float4* bias4 = BIAS ? reinterpret_cast<const float4*>(p.keys.bias + b * p.keys.bias_pitch + key0 + 64 * half) : nullptr;
+      const int64_t left64 = keys - key0;
+      const int left = left64 < BN ? static_cast<int>(left64) : BN;  // keys of this tile up to the last one
+      // one bit per key of this half that takes part (with a bias: per key up to the last one)
+      uint32_t bits[2] = {0xffffffffu, 0xffffffffu};
+      bool used = row < left;  // the key of this row's number
+      if (left < BN) {
 #pragma unroll
-      for (int w = 0; w < 4; ++w) {
-        const int64_t n = left - 32 * w;
-        bits[w] = n >= 32 ? 0xffffffffu : n <= 0 ? 0u : (1u << n) - 1u;
-      }
-      if (!BIAS && p.keys.mask != nullptr) {
-#pragma unroll
-        for (int w = 0; w < 4; ++w) {
-          const bool in = 32 * w + lane < left &&
-                          __ldg(p.keys.mask + b * p.keys.mask_b + (key0 + 32 * w + lane) * p.keys.mask_k) != 0;
-          bits[w] = __ballot_sync(0xffffffffu, in);
+        for (int w = 0; w < 2; ++w) {
+          const int n = left - 64 * half - 32 * w;
+          bits[w] = n >= 32 ? 0xffffffffu : n <= 0 ? 0u : (1u << n) - 1u;
         }
       }
-      {  // wide: both tiles clear the same rows, each before its own second product
-        const uint32_t mine = quarter == 0 ? bits[0] : quarter == 1 ? bits[1] : quarter == 2 ? bits[2] : bits[3];
-        bool clear = !((mine >> lane) & 1) && key0 + row < p.kv_len;
-        if (BIAS && !clear) clear = row < left && __ldg(reinterpret_cast<const float*>(bias4) + row) == -INFINITY;
-        if (__any_sync(0xffffffffu, clear)) {
-          const int i = v_load(t, j);
-          if (!(good = wait(&sh.full[i % L::STAGES], (i / L::STAGES) & 1))) break;
-          if (clear) {
-            uint4* v = reinterpret_cast<uint4*>(sKV + (i % L::STAGES) * L::TILE_BYTES + row * 128);
+      if (BIAS) {
+        used = used && __ldg(p.keys.bias + b * p.keys.bias_pitch + key0 + row) != -INFINITY;
+      } else if (p.keys.mask != nullptr) {
+        const uint8_t* mask = p.keys.mask + b * p.keys.mask_b;
+        used = used && __ldg(mask + (key0 + row) * p.keys.mask_k) != 0;
 #pragma unroll
-            for (int c = 0; c < L::BLOCKS; ++c)
-#pragma unroll
-              for (int e = 0; e < 8; ++e) v[c * (L::BLOCK_BYTES / 16) + e] = make_uint4(0, 0, 0, 0);
-          }
-          fence_proxy_async_smem();
+        for (int w = 0; w < 2; ++w) {
+          const int i = 64 * half + 32 * w + lane;
+          bits[w] = __ballot_sync(0xffffffffu, i < left && __ldg(mask + (key0 + i) * p.keys.mask_k) != 0);
         }
       }
-      if (!(good = wait(&sh.s_full[t], j & 1))) break;
+      const bool clear = !used && key0 + row < p.kv_len;
+      if (__any_sync(0xffffffffu, clear)) {
+        // wide: both tiles clear the same rows, each before its own second product
+        const int i = v_load(t, j);
+        wait(&sh.full[i % L::STAGES], (i / L::STAGES) & 1);
+        if (clear && good) {
+          uint4* v = reinterpret_cast<uint4*>(sKV + (i % L::STAGES) * L::TILE_BYTES + row * 128 +
+                                              half * (DP == 128 ? L::BLOCK_BYTES : 64));
+#pragma unroll
+          for (int e = 0; e < DP / 16; ++e) v[e] = make_uint4(0, 0, 0, 0);
+        }
+        fence_proxy_async_smem();
+      }
+      wait(&sh.s_full[t], j & 1);
       tc_fence_after();
       if (live) {
-        uint32_t r[BN];
-#pragma unroll
-        for (int c = 0; c < BN; c += 32) tmem_ld_32x32b_x32(t_s + c, *reinterpret_cast<uint32_t(*)[32]>(r + c));
+        uint32_t r[64];
+        tmem_ld_32x32b_x32(t_s + 64 * half, *reinterpret_cast<uint32_t(*)[32]>(r));
+        tmem_ld_32x32b_x32(t_s + 64 * half + 32, *reinterpret_cast<uint32_t(*)[32]>(r + 32));
         tmem_ld_wait();
-#pragma unroll
-        for (int c = 0; c < BN; c += 32) reg_dep32(*reinterpret_cast<uint32_t(*)[32]>(r + c));
+        reg_dep32(*reinterpret_cast<uint32_t(*)[32]>(r));
+        reg_dep32(*reinterpret_cast<uint32_t(*)[32]>(r + 32));
         float* y = reinterpret_cast<float*>(r);
         if (BIAS) {
 #pragma unroll
-          for (int e = 0; e < BN; e += 4) {
+          for (int e = 0; e < 64; e += 4) {
             // an excluded key's score may be NaN; behind the last key the bias row may have ended
             const float4 a = (bits[e / 32] >> (e & 31)) & 1 ? __ldg(bias4 + e / 4)
                                                             : make_float4(-INFINITY, -INFINITY, -INFINITY, -INFINITY);
@@ -462,19 +461,25 @@ tile_kernel(const __grid_constant__ CUtensorMap tq, const __grid_constant__ CUte
             y[e + 2] = a.z == -INFINITY ? -INFINITY : fmaf(y[e + 2], scale2, a.z);
             y[e + 3] = a.w == -INFINITY ? -INFINITY : fmaf(y[e + 3], scale2, a.w);
           }
-        } else if ((bits[0] & bits[1] & bits[2] & bits[3]) != 0xffffffffu) {
+        } else if ((bits[0] & bits[1]) != 0xffffffffu) {
 #pragma unroll
-          for (int e = 0; e < BN; ++e) y[e] = (bits[e / 32] >> (e & 31)) & 1 ? y[e] : -INFINITY;
+          for (int e = 0; e < 64; ++e) y[e] = (bits[e / 32] >> (e & 31)) & 1 ? y[e] : -INFINITY;
         }
         float mx[4] = {y[0], y[1], y[2], y[3]};
 #pragma unroll
-        for (int e = 4; e < BN - 4; e += 8) {
+        for (int e = 4; e < 60; e += 8) {
 #pragma unroll
           for (int u = 0; u < 4; ++u) mx[u] = fmax3(mx[u], y[e + u], y[e + 4 + u]);
         }
 #pragma unroll
-        for (int u = 0; u < 4; ++u) mx[u] = fmaxf(mx[u], y[BN - 4 + u]);
-        const float top = fmaxf(fmax3(mx[0], mx[1], mx[2]), mx[3]);
+        for (int u = 0; u < 4; ++u) mx[u] = fmaxf(mx[u], y[60 + u]);
+        float top = fmaxf(fmax3(mx[0], mx[1], mx[2]), mx[3]);
+        // the other half's maximum (it is read before that half's arrival at p_full, so the next step's
+        // value cannot overtake it); the barrier also lets a half write its weights over the scores that
+        // the other has read by now
+        sh.x[t][half][row] = top;
+        named_barrier(3 + 4 * t + quarter, 64);
+        top = fmaxf(top, sh.x[t][half ^ 1][row]);
         const float m_new = fmaxf(m, BIAS ? top : top * scale2);
         if (j == 0) {
           m = m_new;
@@ -482,42 +487,42 @@ tile_kernel(const __grid_constant__ CUtensorMap tq, const __grid_constant__ CUte
           const float alpha = m_new == -INFINITY ? 1.0f : ex2_approx(m - m_new);
           m = m_new;
           l2 = mul2(l2, make_float2(alpha, alpha));
-          if (!(good = wait(&sh.o_full[t], (j - 1) & 1))) break;
+          wait(&sh.o_full[t], (j - 1) & 1);
           tc_fence_after();
 #pragma unroll 1
-          for (int c = 0; c < DP; c += 32) {
-            uint32_t r[32];
-            tmem_ld_32x32b_x32(t_o + c, r);
+          for (int c = 0; c < DP / 2; c += 16) {
+            uint32_t o[16];
+            tmem_ld_32x32b_x16(t_o + c, o);
             tmem_ld_wait();
-            reg_dep32(r);
+            reg_dep16(o);
 #pragma unroll
-            for (int e = 0; e < 32; ++e) r[e] = __float_as_uint(__uint_as_float(r[e]) * alpha);
-            tmem_st_32x32b_x32(t_o + c, r);
+            for (int e = 0; e < 16; ++e) o[e] = __float_as_uint(__uint_as_float(o[e]) * alpha);
+            tmem_st_32x32b_x16(t_o + c, o);
           }
         }
         const float off = m == -INFINITY ? 0.0f : -m;
         const float sc = BIAS ? 1.0f : scale2;
         const float2 off2 = make_float2(off, off), sc2 = make_float2(sc, sc);
 #pragma unroll
-        for (int half = 0; half < 2; ++half) {
-          uint32_t w[32];
-          weights<T>(y + 64 * half, sc2, off2, l2, w);
-          tmem_st_32x32b_x32(t_s + 32 * half, w);
-          tmem_st_wait();
-          tc_fence_before();
-          __syncwarp();
-          if (lane == 0) mbar_arrive(&sh.p_full[t][half]);
+        for (int c = 0; c < 64; c += 32) {
+          uint32_t w[16];
+          weights<T>(y + c, sc2, off2, l2, w);
+          tmem_st_32x32b_x16(t_s + 32 * half + c / 2, w);
         }
-      } else {
-        __syncwarp();
-        if (lane < 2) mbar_arrive(&sh.p_full[t][lane]);
+        tmem_st_wait();
       }
+      tc_fence_before();
+      __syncwarp();
+      if (lane == 0) mbar_arrive(&sh.p_full[t]);
     }
-    const float l = l2.x + l2.y;
-    if (good && steps > 0) {
-      good = wait(&sh.o_full[t], (steps - 1) & 1);
+    if (steps > 0) {
+      wait(&sh.o_full[t], (steps - 1) & 1);
       tc_fence_after();
     }
+    // the sum over both halves
+    sh.x[t][half][row] = l2.x + l2.y;
+    named_barrier(3 + 4 * t + quarter, 64);
+    const float l = sh.x[t][0][row] + sh.x[t][1][row];
     if (SPLIT) {
       // (m, l) and O of this piece; O stays unwritten where no key took part
       if (good && !sh.abort && live) {
@@ -526,11 +531,11 @@ tile_kernel(const __grid_constant__ CUtensorMap tq, const __grid_constant__ CUte
         const int64_t at = ((2 * split + t) * items + item) * p.rows + row;
         const int64_t parts = 2 * p.splits;
         const bool exists = row < p.rows;
-        if (exists) reinterpret_cast<float2*>(p.partial)[at] = make_float2(m, l);
+        if (exists && half == 0) reinterpret_cast<float2*>(p.partial)[at] = make_float2(m, l);
         if (steps > 0) {
-          float* o = p.partial + 2 * parts * items * p.rows + at * DP;
+          float* o = p.partial + 2 * parts * items * p.rows + at * DP + half * (DP / 2);
 #pragma unroll 1
-          for (int c = 0; c < DP; c += 32) {
+          for (int c = 0; c < DP / 2; c += 32) {
             uint32_t r[32];
             tmem_ld_32x32b_x32(t_o + c, r);
             tmem_ld_wait();
@@ -549,7 +554,7 @@ tile_kernel(const __grid_constant__ CUtensorMap tq, const __grid_constant__ CUte
       if (good) {
         const float inv = l == 0.0f ? 0.0f : 1.0f / l;
 #pragma unroll 1
-        for (int c = 0; c < DP; c += 32) {
+        for (int c = 0; c < DP / 2; c += 32) {
           uint32_t r[32];
           if (steps > 0) {
             tmem_ld_32x32b_x32(t_o + c, r);
@@ -559,21 +564,22 @@ tile_kernel(const __grid_constant__ CUtensorMap tq, const __grid_constant__ CUte
 #pragma unroll
             for (int e = 0; e < 32; ++e) r[e] = 0;
           }
-          uint8_t* dst = stage + (c >> 6) * L::BLOCK_BYTES + row * 128;
+          const int col = half * (DP / 2) + c;
+          uint8_t* dst = stage + (col >> 6) * L::BLOCK_BYTES + row * 128;
 #pragma unroll
           for (int u = 0; u < 4; ++u) {
             uint32_t w[4];
 #pragma unroll
             for (int e = 0; e < 4; ++e)
               w[e] = pack2<T>(__uint_as_float(r[8 * u + 2 * e]) * inv, __uint_as_float(r[8 * u + 2 * e + 1]) * inv);
-            const int chunk = ((c & 63) >> 3) + u;
+            const int chunk = ((col & 63) >> 3) + u;
             *reinterpret_cast<uint4*>(dst + ((chunk ^ (row & 7)) << 4)) = make_uint4(w[0], w[1], w[2], w[3]);
           }
         }
         fence_proxy_async_smem();
       }
-      named_barrier(1 + t, BM);  // reached on every path
-      if (good && !sh.abort && quarter == 0 && lane == 0) {
+      named_barrier(1 + t, 2 * BM);  // reached on every path
+      if (good && !sh.abort && quarter == 0 && half == 0 && lane == 0) {
         for (int c = 0; c < L::BLOCKS; ++c)
           tma_store_4d(&to, stage + c * L::BLOCK_BYTES, c * 64, hk * p.group, static_cast<int32_t>(tok0 + t * p.tokens), b);
         bulk_commit_group();
@@ -584,7 +590,7 @@ tile_kernel(const __grid_constant__ CUtensorMap tq, const __grid_constant__ CUte
   }
   tc_fence_before();
   __syncthreads();
-  if (warp == 9) {
+  if (warp == WARP_MMA) {
     tc_fence_after();
     tmem_dealloc(tmem, 512);
   }

@@ -28,6 +28,7 @@ enum DeviceError : unsigned int {
   kErrWaitTimeoutEpilogue = 3,
   kErrWaitTimeoutDrain = 4,
   kErrTmemAlloc = 5,
+  kErrSmemAlign = 6,
 };
 
 __device__ __forceinline__ void record_error(unsigned int code) {
