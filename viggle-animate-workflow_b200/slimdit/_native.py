@@ -230,6 +230,35 @@ def stream_ptr(torch_mod, device=None) -> int:
     return torch_mod.cuda.current_stream(device).cuda_stream
 
 
+def raw_stream(device) -> int:
+    """The current stream of a CUDA device as an integer."""
+    import torch
+
+    get = getattr(torch._C, "_cuda_getCurrentRawStream", None)  # a Stream object costs 2 us
+    if get is None or device.index is None:
+        return torch.cuda.current_stream(device).cuda_stream
+    return get(device.index)
+
+
+class on_device:
+    """torch.cuda.device(device) that does nothing when the device is already the current one."""
+
+    __slots__ = ("ctx",)
+
+    def __init__(self, device):
+        import torch
+
+        self.ctx = None if device.index == torch.cuda.current_device() else torch.cuda.device(device)
+
+    def __enter__(self):
+        if self.ctx is not None:
+            self.ctx.__enter__()
+
+    def __exit__(self, *exc):
+        if self.ctx is not None:
+            self.ctx.__exit__(*exc)
+
+
 def device_error() -> int:
     """Synchronise and return (then clear) the kernels' device error word (0 = none)."""
     code = ctypes.c_uint(0)

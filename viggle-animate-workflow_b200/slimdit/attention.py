@@ -23,8 +23,14 @@ import ctypes
 import dataclasses
 import time
 
+import torch
+
+from . import _native as nat
+from .ops import _no_grad, _view
+
 DEFAULT_MIN_SEQ = 12000  # below this the dense path wins outright (attention_triton.py:34)
 HEAD_DIM = 128  # the one head dim the kernel supports (MiniMax-H3: 56 heads x 128)
+_MASK_TYPES = {torch.float32: nat.F32, torch.bfloat16: nat.BF16, torch.float16: nat.F16, torch.bool: nat.MASK_BOOL}
 
 
 def unwrap(value):
@@ -236,21 +242,20 @@ def attention_heads(qkv, heads: int, rank: int, world: int, rotate: bool = True,
 def _cross_rows(t, name: str, shared: bool):
     """[S, H, D] or [B, S, H, D] as a 4-D view of 16-byte aligned rows (copied when it is not one);
     ``shared``: strides of 0 may stay for the batch and the heads."""
-    import torch
-
     if not isinstance(t, torch.Tensor) or not t.is_cuda:
+        nat.require_cuda()
         raise TypeError(f"{name} must be a CUDA tensor")
-    if t.dtype not in (torch.bfloat16, torch.float16):
+    if t.dtype != torch.bfloat16 and t.dtype != torch.float16:
         raise TypeError(f"cross attention takes bf16 or fp16 tensors, got {t.dtype} {name}")
-    if t.dim() not in (3, 4):
-        raise ValueError(f"expected [tokens, heads, dim] or [batch, tokens, heads, dim] {name}, got {tuple(t.shape)}")
-    if t.dim() == 3:
+    n = t.dim()
+    if n != 4:
+        if n != 3:
+            raise ValueError(f"expected [tokens, heads, dim] or [batch, tokens, heads, dim] {name}, got {tuple(t.shape)}")
         t = t.unsqueeze(0)
     b, s, h, d = t.shape
-    st = t.stride()
-    if ((d > 1 and st[3] != 1) or t.data_ptr() % 16 or (b > 1 and st[0] % 8) or (s > 1 and st[1] % 8)
-            or (h > 1 and st[2] % 8) or (s > 1 and st[1] == 0)
-            or (not shared and ((b > 1 and st[0] == 0) or (h > 1 and st[2] == 0)))):
+    sb, ss, sh, sd = t.stride()
+    if ((d > 1 and sd != 1) or t.data_ptr() & 15 or (b > 1 and sb & 7) or (s > 1 and (ss & 7 or ss == 0))
+            or (h > 1 and sh & 7) or (not shared and ((b > 1 and sb == 0) or (h > 1 and sh == 0)))):
         t = t.clone(memory_format=torch.contiguous_format)
     return t
 
@@ -269,54 +274,53 @@ def cross_attention(q, k, v, key_mask=None, kv_lengths=None, scale: float | None
     apply. What stands in excluded keys and values, NaN included, has no influence; a row without keys
     is 0. scale: D^-0.5 if not given. Scores, maxima and sums are fp32; the weights are rounded to the
     type of v for the second product. Inference only: there is no backward pass."""
-    from . import _native as nat
-    from .ops import _no_grad, _view
-
-    torch = nat.require_cuda()
-    _no_grad(q, k, v, key_mask if isinstance(key_mask, torch.Tensor) else None)
     q4, k4, v4 = _cross_rows(q, "q", False), _cross_rows(k, "k", True), _cross_rows(v, "v", True)
+    _no_grad(q, k, v, key_mask)
     if k.dim() != q.dim() or v.dim() != q.dim():
         raise ValueError("q, k and v must have the same number of dimensions")
     b, sq, h, d = q4.shape
-    sk, hk = k4.shape[1:3]
-    dev = q4.device
-    if k4.dtype != q4.dtype or v4.dtype != q4.dtype or k4.device != dev or v4.device != dev:
+    bk, sk, hk, dk = k4.shape
+    dev, dtype = q4.device, q4.dtype
+    if k4.dtype != dtype or v4.dtype != dtype or k4.device != dev or v4.device != dev:
         raise ValueError("q, k and v must have one dtype and one device")
-    if k4.shape != v4.shape or k4.shape[0] != b or k4.shape[3] != d:
+    if k4.shape != v4.shape or bk != b or dk != d:
         raise ValueError(f"k {tuple(k.shape)} and v {tuple(v.shape)} do not fit q {tuple(q.shape)}")
-    mask_type, mask_b, mask_k = 0, 0, 0
+    mask_ptr, mask_type, mask_b, mask_k, additive = None, 0, 0, 0, 0
     if key_mask is not None:
-        types = {torch.float32: nat.F32, torch.bfloat16: nat.BF16, torch.float16: nat.F16, torch.bool: nat.MASK_BOOL}
-        if not isinstance(key_mask, torch.Tensor) or key_mask.dtype not in types:
+        if not isinstance(key_mask, torch.Tensor) or key_mask.dtype not in _MASK_TYPES:
             raise TypeError("key_mask must be a bool, fp32, bf16 or fp16 tensor")
         if key_mask.device != dev:
             raise ValueError("key_mask must be on the device of q")
         m = key_mask[:, 0, 0] if key_mask.dim() == 4 and key_mask.shape[1:3] == (1, 1) else key_mask
-        if tuple(m.shape) not in ((sk,), (b, sk), (1, sk)):
+        if not 1 <= m.dim() <= 2 or m.shape[-1] != sk or (m.dim() == 2 and m.shape[0] not in (1, b)):
             raise ValueError(f"key_mask {tuple(key_mask.shape)} does not fit {b} x {sk} keys (masks per query are not "
                              "supported)")
-        mask_type, mask_k = types[m.dtype], m.stride(-1)
+        mask_ptr, mask_type, mask_k = m.data_ptr(), _MASK_TYPES[m.dtype], m.stride(-1)
         mask_b = m.stride(0) if m.dim() == 2 and m.shape[0] == b and b > 1 else 0
+        additive = 1 if mask_type != nat.MASK_BOOL else 0
+    len_ptr, len_bits = None, 0
     if kv_lengths is not None:
         if not isinstance(kv_lengths, torch.Tensor) or kv_lengths.dtype not in (torch.int32, torch.int64):
             raise TypeError("kv_lengths must be an int32 or int64 tensor")
-        if kv_lengths.device != dev or tuple(kv_lengths.shape) != (b,):
+        if kv_lengths.device != dev or kv_lengths.dim() != 1 or kv_lengths.shape[0] != b:
             raise ValueError(f"kv_lengths must be [{b}] on the device of q")
         kv_lengths = kv_lengths.contiguous()
-    scale = max(d, 1) ** -0.5 if scale is None else float(scale)
+        len_ptr, len_bits = kv_lengths.data_ptr(), 64 if kv_lengths.dtype == torch.int64 else 32
+    if scale is None:
+        scale = max(d, 1) ** -0.5
     lib = nat.load()
-    out = torch.empty((b, sq, h, d), dtype=q4.dtype, device=dev)
-    additive = key_mask is not None and key_mask.dtype != torch.bool
+    out = torch.empty_like(q4, memory_format=torch.contiguous_format)
     need = ctypes.c_uint64(0)
-    with torch.cuda.device(dev):
-        nat.check(lib.slim_cross_attn_workspace_bytes(b, sq, sk, h, hk, d, int(additive), ctypes.byref(need)))
-        ws = torch.empty((need.value,), dtype=torch.uint8, device=dev) if need.value else None
-        nat.check(lib.slim_cross_attn(
-            _view(q4), _view(k4), _view(v4), _view(out), nat.BF16 if q4.dtype == torch.bfloat16 else nat.F16, b, sq, sk,
-            h, hk, d, None if key_mask is None else m.data_ptr(), mask_type, mask_b, mask_k,
-            None if kv_lengths is None else kv_lengths.data_ptr(),
-            0 if kv_lengths is None else 64 if kv_lengths.dtype == torch.int64 else 32, scale,
-            None if ws is None else ws.data_ptr(), need.value, torch.cuda.current_stream(dev).cuda_stream))
+    with nat.on_device(dev):
+        nat.check(lib.slim_cross_attn_workspace_bytes(b, sq, sk, h, hk, d, additive, need))
+        ws, ws_ptr = None, None
+        if need.value:
+            ws = torch.empty((need.value,), dtype=torch.uint8, device=dev)
+            ws_ptr = ws.data_ptr()
+        nat.check(lib.slim_cross_attn(_view(q4), _view(k4), _view(v4), _view(out),
+                                      nat.BF16 if dtype == torch.bfloat16 else nat.F16, b, sq, sk, h, hk, d, mask_ptr,
+                                      mask_type, mask_b, mask_k, len_ptr, len_bits, float(scale), ws_ptr, need.value,
+                                      nat.raw_stream(dev)))
     return out if q.dim() == 4 else out[0]
 
 

@@ -526,21 +526,26 @@ _LAYOUTS = {"half": nat.ROTARY_HALF, "interleaved": nat.ROTARY_INTERLEAVED}
 
 def _no_grad(*tensors) -> None:
     """The kernels record no gradient: refuse tensors that expect one instead of dropping it."""
-    if torch.is_grad_enabled() and any(t is not None and t.requires_grad for t in tensors):
-        raise ValueError("this operator has no backward pass; call it under torch.no_grad() or detach its inputs")
+    if not torch.is_grad_enabled():
+        return
+    for t in tensors:
+        if t is not None and t.requires_grad:
+            raise ValueError("this operator has no backward pass; call it under torch.no_grad() or detach its inputs")
 
 
 def _rows4(t: torch.Tensor, name: str, inplace: bool) -> torch.Tensor:
     """[S, H, D] or [B, S, H, D] as a 4-D view with consecutive elements in each row."""
     if not isinstance(t, torch.Tensor) or not t.is_cuda:
+        nat.require_cuda()
         raise TypeError(f"{name} must be a CUDA tensor")
     if t.dtype not in _DT:
         raise TypeError(f"unsupported dtype {t.dtype}")
-    if t.dim() not in (3, 4):
-        raise ValueError(f"expected [tokens, heads, dim] or [batch, tokens, heads, dim] {name}, got {tuple(t.shape)}")
-    if t.dim() == 3:
+    n = t.dim()
+    if n != 4:
+        if n != 3:
+            raise ValueError(f"expected [tokens, heads, dim] or [batch, tokens, heads, dim] {name}, got {tuple(t.shape)}")
         t = t.unsqueeze(0)
-    if t.shape[3] > 1 and t.stride(3) != 1:
+    if t.stride(3) != 1 and t.shape[3] > 1:
         if inplace:
             raise ValueError(f"{name} needs unit stride in its last dimension to be rotated in place")
         t = t.contiguous()
@@ -595,44 +600,50 @@ def rotary(q: torch.Tensor, k: torch.Tensor | None, positions: torch.Tensor, inv
     2j + 1. ``inverse`` turns by the opposite angles (with 1/magnitude it undoes the rotation).
     Returns (q', k'), or q' alone when k is None: new contiguous tensors, or q and k themselves with
     ``inplace``. The angle is reduced in fp64, the products are fp32, rounded once."""
-    nat.require_cuda()
-    _no_grad(q, k)
     if layout not in _LAYOUTS:
         raise ValueError(f"layout must be one of {sorted(_LAYOUTS)}")
     q4 = _rows4(q, "q", inplace)
+    _no_grad(q, k)
     b, s, h, d = q4.shape
-    dev = q4.device
-    k4 = None
+    dev, dtype = q4.device, q4.dtype
+    k4, hk = None, 0
     if k is not None:
-        if isinstance(k, torch.Tensor) and k.dim() != q.dim():
-            raise ValueError("q and k must have the same number of dimensions")
         k4 = _rows4(k, "k", inplace)
-        if k4.dtype != q4.dtype or k4.device != dev:
+        if k.dim() != q.dim():
+            raise ValueError("q and k must have the same number of dimensions")
+        if k4.dtype != dtype or k4.device != dev:
             raise ValueError("q and k must have one dtype and one device")
-        if k4.shape[:2] != (b, s) or k4.shape[3] != d:
+        bk, sk, hk, dk = k4.shape
+        if bk != b or sk != s or dk != d:
             raise ValueError(f"k {tuple(k.shape)} does not fit q {tuple(q.shape)}")
-    if h == 0 or d == 0 or (k4 is not None and k4.shape[2] == 0):
+    if h == 0 or d == 0 or (k4 is not None and hk == 0):
         raise ValueError("q and k need at least one head and one element")
     if not isinstance(inv_freq, torch.Tensor) or inv_freq.dim() != 1:
         raise ValueError("inv_freq must be a 1-D tensor")
-    if 2 * inv_freq.numel() > d or inv_freq.numel() == 0:
-        raise ValueError(f"{inv_freq.numel()} frequencies do not fit a head of {d} elements")
-    freq = inv_freq.to(device=dev, dtype=torch.float32).contiguous()
+    pairs = inv_freq.shape[0]
+    if 2 * pairs > d or pairs == 0:
+        raise ValueError(f"{pairs} frequencies do not fit a head of {d} elements")
+    freq = inv_freq
+    if freq.dtype != torch.float32 or freq.device != dev or not freq.is_contiguous():
+        freq = freq.to(device=dev, dtype=torch.float32).contiguous()
     if not isinstance(positions, torch.Tensor) or positions.dtype not in (torch.int32, torch.int64):
         raise TypeError("positions must be an int32 or int64 tensor")
     if positions.device != dev:
         raise ValueError("positions must be on the device of q")
-    axes = 1 if sections is None else len(sections)
-    if sections is not None and (not 1 <= axes <= nat.ROTARY_MAX_AXES or any(n < 0 for n in sections)
-                                 or sum(sections) != freq.numel()):
-        raise ValueError(f"sections {tuple(sections)} do not divide {freq.numel()} pairs")
-    shape = tuple(positions.shape) if sections is None else tuple(positions.shape[:-1])
-    if shape not in ((s,), (b, s), (1, s)) or (sections is not None and positions.shape[-1:] != (axes,)):
+    axes, sec = 1, None
+    shape, ps, pos_a = positions.shape, positions.stride(), 0
+    if sections is not None:
+        axes = len(sections)
+        if not 1 <= axes <= nat.ROTARY_MAX_AXES or any(n < 0 for n in sections) or sum(sections) != pairs:
+            raise ValueError(f"sections {tuple(sections)} do not divide {pairs} pairs")
+        sec = (nat.ctypes.c_int * axes)(*sections)
+        if not shape or shape[-1] != axes:
+            raise ValueError(f"positions {tuple(shape)} do not fit {axes} axes")
+        pos_a, shape, ps = ps[-1], shape[:-1], ps[:-1]
+    lead = len(shape)
+    if not 1 <= lead <= 2 or shape[-1] != s or (lead == 2 and shape[0] not in (1, b)):
         raise ValueError(f"positions {tuple(positions.shape)} do not fit {b} x {s} tokens and {axes} axes")
-    ps = positions.stride()
-    pos_a = ps[-1] if sections is not None else 0
-    pos_s = ps[len(shape) - 1]
-    pos_b = ps[0] if len(shape) == 2 and shape[0] == b and b > 1 else 0
+    pos_b = ps[0] if lead == 2 and shape[0] == b and b > 1 else 0
     if inplace:
         for name, t in (("q", q4), ("k", k4)):
             if t is not None and t.numel() and _spans_overlap(t):
@@ -641,17 +652,15 @@ def rotary(q: torch.Tensor, k: torch.Tensor | None, positions: torch.Tensor, inv
             raise ValueError("q and k may share memory: rotate them in place in two calls")
         q_out, k_out = q4, k4
     else:
-        q_out = torch.empty((b, s, h, d), dtype=q4.dtype, device=dev)
-        k_out = None if k4 is None else torch.empty(k4.shape, dtype=q4.dtype, device=dev)
-    qv, qo = _view(q4), _view(q_out)
+        q_out = torch.empty_like(q4, memory_format=torch.contiguous_format)
+        k_out = None if k4 is None else torch.empty_like(k4, memory_format=torch.contiguous_format)
     kv, ko = (None, None) if k4 is None else (_view(k4), _view(k_out))
-    sec = None if sections is None else (nat.ctypes.c_int * axes)(*sections)
-    with torch.cuda.device(dev):
-        nat.check(nat.load().slim_rotary(qv, qo, h, kv, ko, 0 if k4 is None else k4.shape[2], _DT[q4.dtype], b, s, d,
-                                         2 * freq.numel(), _LAYOUTS[layout], positions.data_ptr(),
-                                         64 if positions.dtype == torch.int64 else 32, pos_b, pos_s, pos_a,
-                                         freq.data_ptr(), sec, axes, float(magnitude), int(bool(inverse)),
-                                         _stream(q4)))
+    with nat.on_device(dev):
+        nat.check(nat.load().slim_rotary(_view(q4), _view(q_out), h, kv, ko, hk, _DT[dtype], b, s, d, 2 * pairs,
+                                         _LAYOUTS[layout], positions.data_ptr(),
+                                         64 if positions.dtype == torch.int64 else 32, pos_b, ps[lead - 1], pos_a,
+                                         freq.data_ptr(), sec, axes, magnitude, 1 if inverse else 0,
+                                         nat.raw_stream(dev)))
     if inplace:
         return q if k is None else (q, k)
     if q.dim() == 3:
