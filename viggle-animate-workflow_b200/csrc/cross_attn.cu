@@ -146,16 +146,18 @@ struct Layout {
   static constexpr int BLOCK_BYTES = 128 * 128;
   static constexpr int TILE_BYTES = BLOCKS * BLOCK_BYTES;
   static constexpr int Q_TILES = SPLIT ? 1 : 2;
-  static constexpr int STAGES = DP == 128 ? 7 - Q_TILES : 8;
+  static constexpr int STAGES = DP == 64 ? 8 : SPLIT ? 6 : 4;
+  static constexpr int STAGING_BYTES = SPLIT ? 0 : 2048;  // a softmax warp's: 32 rows x 32 columns of the output
   static constexpr int OFF_KV = Q_TILES * TILE_BYTES;
-  static constexpr int OFF_SH = OFF_KV + STAGES * TILE_BYTES;
+  static constexpr int OFF_STAGING = OFF_KV + STAGES * TILE_BYTES;
+  static constexpr int OFF_SH = OFF_STAGING + SOFTMAX_WARPS * STAGING_BYTES;
 };
 
 template <int STAGES>
 struct Shared {
-  uint64_t q_full[2];
+  uint64_t q_full[2], q_free[2];
   uint64_t full[STAGES], empty[STAGES];
-  uint64_t s_full[2], p_full[2], o_full[2];
+  uint64_t s_full[2], p_full[2], o_full[2], o_free[2];
   uint64_t turn[2];   // wide: the tile whose MMAs may be issued
   uint64_t drain[2];
   uint32_t tmem_base;
@@ -170,16 +172,45 @@ constexpr size_t smem_bytes() {
 }
 
 struct TileParams {
+  slim_view out;
   int64_t q_len, kv_len;
+  int kv_heads, dim;
   int group, tokens;          // query heads per key head, tokens per 128-row tile
   int kb, kh, vb, vh;         // 0 for a k / v that is the same for every sequence / head
   float scale2;
   Keys keys;
+  int items, per_head;        // items in all, and of one (sequence, key head)
   // SPLIT
-  int splits, per;            // CTAs per tile of rows, key tiles of each (even)
+  int splits, per;            // items per tile of rows, key tiles of each (even)
   int rows;                   // rows of a tile that exist
   float* partial;
 };
+
+// One piece of work: a pair of row tiles (SPLIT: one row tile and a range of the keys) of a (sequence, head).
+struct Item {
+  int b, hk, split, tiles;
+  int64_t q_tile, tok0, keys;
+  int j0, steps;              // SPLIT: first key tile; steps over key tiles
+};
+
+template <bool BIAS, bool SPLIT>
+__device__ __forceinline__ Item item_at(const TileParams& p, int index) {
+  Item it;
+  const int head = index / p.per_head, x = index - head * p.per_head;
+  it.b = head / p.kv_heads;
+  it.hk = head - it.b * p.kv_heads;
+  it.split = SPLIT ? x % p.splits : 0;
+  it.q_tile = SPLIT ? x / p.splits : 2 * static_cast<int64_t>(x);
+  it.tok0 = it.q_tile * p.tokens;
+  it.tiles = SPLIT || it.tok0 + p.tokens < p.q_len ? 2 : 1;
+  it.keys = BIAS ? p.keys.n_keys[it.b]
+            : p.keys.lengths != nullptr ? clamp_length(p.keys.lengths, p.keys.lengths64, it.b, p.kv_len)
+                                        : p.kv_len;
+  const int nk = static_cast<int>((it.keys + BN - 1) / BN);
+  it.j0 = SPLIT ? it.split * p.per : 0;
+  it.steps = !SPLIT ? nk : nk <= it.j0 ? 0 : ((nk - it.j0 < p.per ? nk - it.j0 : p.per) + 1) / 2;
+  return it;
+}
 
 // Partial results of `parts` pieces of `items` tiles of `rows` rows: (m, l) pairs, then O rows.
 __host__ __device__ inline int64_t split_floats(int64_t parts, int64_t items, int64_t rows, int dp) {
@@ -216,12 +247,13 @@ __device__ __forceinline__ void weights(const float* y, float2 sc2, float2 off2,
 template <typename T, int DP, bool BIAS, bool SPLIT>
 __global__ void __launch_bounds__(THREADS, 1)
 tile_kernel(const __grid_constant__ CUtensorMap tq, const __grid_constant__ CUtensorMap tk,
-            const __grid_constant__ CUtensorMap tv, const __grid_constant__ CUtensorMap to, const TileParams p) {
+            const __grid_constant__ CUtensorMap tv, const TileParams p) {
   using L = Layout<DP, SPLIT>;
   using Sh = Shared<L::STAGES>;
   constexpr bool BF16 = std::is_same<T, __nv_bfloat16>::value;
   constexpr uint32_t IDESC_QK = idesc_f16(BM, BN, BF16, false);
   constexpr uint32_t IDESC_PV = idesc_f16(BM, DP, BF16, true);
+  constexpr int STEP_LOADS = SPLIT ? 4 : 2;
   extern __shared__ __align__(1024) uint8_t tile_smem[];
   uint8_t* smem = tile_smem;
   if (smem_u32(smem) & 1023) {  // the swizzled tiles need it; there is no room to round up
@@ -234,35 +266,25 @@ tile_kernel(const __grid_constant__ CUtensorMap tq, const __grid_constant__ CUte
 
   const int warp = threadIdx.x >> 5;
   const int lane = threadIdx.x & 31;
-  const int b = blockIdx.z, hk = blockIdx.y;
-  const int split = SPLIT ? static_cast<int>(blockIdx.x % p.splits) : 0;
-  const int64_t q_tile = SPLIT ? blockIdx.x / p.splits : 2 * static_cast<int64_t>(blockIdx.x);
-  const int64_t tok0 = q_tile * p.tokens;
-  const int tiles = SPLIT || tok0 + p.tokens < p.q_len ? 2 : 1;
-  const int64_t keys = BIAS ? p.keys.n_keys[b]
-                       : p.keys.lengths != nullptr ? clamp_length(p.keys.lengths, p.keys.lengths64, b, p.kv_len)
-                                                   : p.kv_len;
-  // key tile of step j: wide, j for both tiles; SPLIT, j0 + 2 j + t
-  const int nk = static_cast<int>((keys + BN - 1) / BN);
-  const int j0 = SPLIT ? split * p.per : 0;
-  const int steps = !SPLIT ? nk : nk <= j0 ? 0 : ((nk - j0 < p.per ? nk - j0 : p.per) + 1) / 2;
-  auto key_tile = [&](int t, int j) { return SPLIT ? j0 + 2 * j + t : j; };
-  // position of a tile's K and V of step j in the order of the loads
-  auto k_load = [](int t, int j) { return SPLIT ? 4 * j + t : 2 * j; };
-  auto v_load = [](int t, int j) { return SPLIT ? 4 * j + 2 + t : 2 * j + 1; };
+  // key tile of a step: wide, j for both tiles; SPLIT, j0 + 2 j + t. Position of a tile's K and V in the
+  // order of a step's loads: wide K V, SPLIT K_0 K_1 V_0 V_1
+  auto k_load = [](int t) { return SPLIT ? t : 0; };
+  auto v_load = [](int t) { return SPLIT ? 2 + t : 1; };
 
   if (threadIdx.x == 0) {
     for (int t = 0; t < 2; ++t) {
       mbar_init(&sh.q_full[t], 1);
+      mbar_init(&sh.q_free[t], SPLIT ? 2 : 1);
       mbar_init(&sh.s_full[t], 1);
       mbar_init(&sh.p_full[t], 2 * BM / 32);
       mbar_init(&sh.o_full[t], 1);
+      mbar_init(&sh.o_free[t], 2 * BM / 32);
       mbar_init(&sh.turn[t], 1);
       mbar_init(&sh.drain[t], 1);
     }
     for (int s = 0; s < L::STAGES; ++s) {
       mbar_init(&sh.full[s], 1);
-      mbar_init(&sh.empty[s], SPLIT ? 1 : tiles);  // wide: both tiles have used it
+      mbar_init(&sh.empty[s], SPLIT ? 1 : 2);  // wide: both tiles have used it
     }
     sh.abort = 0;
     fence_mbar_init();
@@ -278,110 +300,143 @@ tile_kernel(const __grid_constant__ CUtensorMap tq, const __grid_constant__ CUte
 
   if (warp >= SOFTMAX_WARPS) {
     regs_dec<REGS_OTHER>();
-  if (warp == WARP_TMA) {
-    // ------------------------------------------------------------ TMA producer
-    if (lane == 0 && steps > 0) {
-      const uint32_t q_bytes = static_cast<uint32_t>(L::BLOCKS * 128 * p.group * p.tokens);
-      const int q_tiles = SPLIT ? 1 : tiles;
-      for (int t = 0; t < q_tiles; ++t) {
-        mbar_arrive_expect_tx(&sh.q_full[t], q_bytes);
-        for (int c = 0; c < L::BLOCKS; ++c)
-          tma_load_4d(sQ + t * L::TILE_BYTES + c * L::BLOCK_BYTES, &tq, &sh.q_full[t], c * 64, hk * p.group,
-                      static_cast<int32_t>(tok0 + t * p.tokens), b);
-      }
-      uint32_t issued = 0, last_parity = 0;
-      const int loads = (SPLIT ? 4 : 2) * steps;
-      for (int i = 0; i < loads && !sh.abort; ++i) {
-        const int s = i % L::STAGES;
-        const uint32_t ph = (i / L::STAGES) & 1;
-        if (!mbar_wait(&sh.empty[s], ph ^ 1, kErrWaitTimeoutProducer)) {
-          sh.abort = 1;
-          break;
+    if (warp == WARP_TMA) {
+      // ---------------------------------------------------------- TMA producer
+      if (lane == 0) {
+        const uint32_t q_bytes = static_cast<uint32_t>(L::BLOCKS * 128 * p.group * p.tokens);
+        uint32_t issued = 0, last_parity = 0;   // per slot
+        uint32_t q_loads[2] = {0, 0};
+        int slot = 0, parity = 0;
+        bool ok = true;
+        auto wait = [&](uint64_t* bar, uint32_t ph) {
+          ok = ok && mbar_wait_abort(bar, ph, kErrWaitTimeoutProducer, &sh.abort);
+          return ok;
+        };
+        auto load = [&](const Item& it, int i) {
+          if (!wait(&sh.empty[slot], parity ^ 1)) return;
+          const bool is_v = SPLIT ? (i & 2) != 0 : (i & 1) != 0;
+          const int kt = SPLIT ? it.j0 + 2 * (i >> 2) + (i & 1) : i >> 1;
+          mbar_arrive_expect_tx(&sh.full[slot], L::TILE_BYTES);
+          for (int c = 0; c < L::BLOCKS; ++c)  // rows past the end come as zeros
+            tma_load_4d(sKV + slot * L::TILE_BYTES + c * L::BLOCK_BYTES, is_v ? &tv : &tk, &sh.full[slot], c * 64,
+                        it.hk * (is_v ? p.vh : p.kh), kt * BN, it.b * (is_v ? p.vb : p.kb));
+          issued |= 1u << slot;
+          last_parity = (last_parity & ~(1u << slot)) | (static_cast<uint32_t>(parity) << slot);
+          if (++slot == L::STAGES) {
+            slot = 0;
+            parity ^= 1;
+          }
+        };
+        for (int index = blockIdx.x; ok && index < p.items; index += gridDim.x) {
+          const Item it = item_at<BIAS, SPLIT>(p, index);
+          if (it.steps == 0) continue;
+          // the first keys do not have to wait for the last item's queries to be done with
+          load(it, 0);
+          const int q_tiles = SPLIT ? 1 : it.tiles;
+          for (int t = 0; ok && t < q_tiles; ++t) {
+            if (q_loads[t] > 0 && !wait(&sh.q_free[t], (q_loads[t] - 1) & 1)) break;
+            mbar_arrive_expect_tx(&sh.q_full[t], q_bytes);
+            for (int c = 0; c < L::BLOCKS; ++c)
+              tma_load_4d(sQ + t * L::TILE_BYTES + c * L::BLOCK_BYTES, &tq, &sh.q_full[t], c * 64, it.hk * p.group,
+                          static_cast<int32_t>(it.tok0 + t * p.tokens), it.b);
+            ++q_loads[t];
+          }
+          for (int i = 1; ok && i < STEP_LOADS * it.steps; ++i) load(it, i);
         }
-        const bool is_v = SPLIT ? (i & 2) != 0 : (i & 1) != 0;
-        const int kt = SPLIT ? key_tile(i & 1, i >> 2) : i >> 1;
-        mbar_arrive_expect_tx(&sh.full[s], L::TILE_BYTES);
-        for (int c = 0; c < L::BLOCKS; ++c)  // rows past the end come as zeros
-          tma_load_4d(sKV + s * L::TILE_BYTES + c * L::BLOCK_BYTES, is_v ? &tv : &tk, &sh.full[s], c * 64,
-                      hk * (is_v ? p.vh : p.kh), kt * BN, b * (is_v ? p.vb : p.kb));
-        issued |= 1u << s;
-        last_parity = (last_parity & ~(1u << s)) | (ph << s);
+        // every load issued by this thread lands before the CTA may exit
+        for (int t = 0; t < 2; ++t)
+          if (q_loads[t] > 0) mbar_wait(&sh.q_full[t], (q_loads[t] - 1) & 1, kErrWaitTimeoutDrain);
+        for (int s = 0; s < L::STAGES; ++s)
+          if (issued & (1u << s)) mbar_wait(&sh.full[s], (last_parity >> s) & 1, kErrWaitTimeoutDrain);
       }
-      // every load issued by this thread lands before the CTA may exit
-      for (int t = 0; t < q_tiles; ++t) mbar_wait(&sh.q_full[t], 0, kErrWaitTimeoutDrain);
-      for (int s = 0; s < L::STAGES; ++s)
-        if (issued & (1u << s)) mbar_wait(&sh.full[s], (last_parity >> s) & 1, kErrWaitTimeoutDrain);
-    }
-  } else if (warp - WARP_MMA < tiles) {
-    // ------------------------------------------------------------ MMA issue of tile t
-    const int t = warp - WARP_MMA;
-    if (lane == 0 && steps > 0) {
-      auto wait = [&](uint64_t* bar, uint32_t parity) { return mbar_wait_abort(bar, parity, kErrWaitTimeoutMma, &sh.abort); };
-      // the ring position of load i, carried along as (slot, parity) instead of dividing
-      struct Ring {
-        int slot, parity;
-        __device__ __forceinline__ Ring at(int n) const {
-          const int s = slot + n;
-          return s >= L::STAGES ? Ring{s - L::STAGES, parity ^ 1} : Ring{s, parity};
-        }
-      };
-      auto full = [&](Ring r) { return wait(&sh.full[r.slot], r.parity); };
-      const uint64_t q_desc = smem_desc_sw128(smem_u32(sQ + (SPLIT ? 0 : t * L::TILE_BYTES)));
-      const uint32_t kv_addr = smem_u32(sKV);
-      const uint32_t t_s = tmem + col_s(t), t_o = tmem + col_o(t);
-      auto qk = [&](Ring r) {
-        const uint64_t kd = smem_desc_sw128(kv_addr + r.slot * L::TILE_BYTES);
+    } else if (warp - WARP_MMA < 2) {
+      // ---------------------------------------------------------- MMA issue of tile t
+      const int t = warp - WARP_MMA;
+      if (lane == 0) {
+        // the ring position of a load, carried along as (slot, parity)
+        struct Ring {
+          int slot, parity;
+          __device__ __forceinline__ Ring at(int n) const {
+            const int s = slot + n;
+            return s >= L::STAGES ? Ring{s - L::STAGES, parity ^ 1} : Ring{s, parity};
+          }
+        };
+        const uint64_t q_desc = smem_desc_sw128(smem_u32(sQ + (SPLIT ? 0 : t * L::TILE_BYTES)));
+        const uint32_t kv_addr = smem_u32(sKV);
+        const uint32_t t_s = tmem + col_s(t), t_o = tmem + col_o(t);
+        Ring base{0, 0};        // of the step's first load
+        uint32_t items = 0;     // of this tile so far
+        uint32_t steps = 0;     // of this tile so far
+        uint32_t batches = 0;   // of MMAs issued in turn so far
+        bool ok = true;
+        auto wait = [&](uint64_t* bar, uint32_t ph) {
+          ok = ok && mbar_poll_abort(bar, ph, kErrWaitTimeoutMma, &sh.abort);
+          return ok;
+        };
+        auto full = [&](Ring r) { return wait(&sh.full[r.slot], r.parity); };
+        for (int index = blockIdx.x; ok && index < p.items; index += gridDim.x) {
+          const Item it = item_at<BIAS, SPLIT>(p, index);
+          if (it.steps == 0) continue;
+          if (t >= it.tiles) {  // the other tile's loads
+            const int n = base.slot + STEP_LOADS * it.steps;
+            base = Ring{n % L::STAGES, base.parity ^ (n / L::STAGES & 1)};
+            continue;
+          }
+          // Both tiles' MMAs share the tensor cores. Issued as they come they interleave, both tiles finish
+          // late and their softmaxes run in step (3.90 instead of 2.77 ms at 16384 x 16111 x 24 heads of
+          // 128); so the batches (second product, next scores) take turns. The turn passes on before a batch's
+          // last MMAs are issued: they cover the time until the other tile's thread has noticed.
+          auto my_turn = [&] { return it.tiles == 1 || wait(&sh.turn[t], t == 0 ? (batches & 1) ^ 1 : batches & 1); };
+          auto pass_turn = [&] {
+            if (it.tiles == 2) {
+              mbar_arrive(&sh.turn[t ^ 1]);
+              ++batches;
+            }
+          };
+          auto qk = [&](Ring r) {
+            const uint64_t kd = smem_desc_sw128(kv_addr + r.slot * L::TILE_BYTES);
 #pragma unroll
-        for (int k = 0; k < DP / 16; ++k) {
-          const uint32_t off = (k >> 2) * L::BLOCK_BYTES + (k & 3) * 32;
-          mma_f16(t_s, smem_desc_at(q_desc, off), smem_desc_at(kd, off), IDESC_QK, k != 0);
-        }
-        mma_commit(&sh.s_full[t]);
-        mma_commit(&sh.empty[r.slot]);
-      };
-      // Both tiles' MMAs share the tensor cores. Issued as they come they interleave, both tiles finish
-      // late and their softmaxes run in step; so each batch (second product, next scores) is issued as
-      // a whole and the tiles take turns.
-      auto my_turn = [&](int k) { return tiles == 1 || wait(&sh.turn[t], t == 0 ? (k & 1) ^ 1 : k & 1); };
-      auto pass_turn = [&] {
-        if (tiles == 2) mbar_arrive(&sh.turn[t ^ 1]);
-      };
-      auto pv = [&](Ring r, int j) {
-        const uint64_t vd = smem_desc_mn_sw128(kv_addr + r.slot * L::TILE_BYTES, L::BLOCK_BYTES);
-        if (!my_turn(j + 1) || !wait(&sh.p_full[t], j & 1)) return false;
-        tc_fence_after();
+            for (int k = 0; k < DP / 16; ++k) {
+              if (k == DP / 32) pass_turn();
+              const uint32_t off = (k >> 2) * L::BLOCK_BYTES + (k & 3) * 32;
+              mma_f16(t_s, smem_desc_at(q_desc, off), smem_desc_at(kd, off), IDESC_QK, k != 0);
+            }
+            mma_commit(&sh.s_full[t]);
+          };
+          if (!full(base.at(k_load(t))) || !wait(&sh.q_full[SPLIT ? 0 : t], items & 1) || !my_turn()) break;
+          tc_fence_after();
+          qk(base.at(k_load(t)));
+          for (int j = 0; j < it.steps; ++j) {
+            const Ring next = base.at(STEP_LOADS), v = base.at(v_load(t)), k = next.at(k_load(t));
+            const bool more = j + 1 < it.steps;
+            if (!full(v) || (more && !full(k)) || !my_turn()) break;
+            // the last item's output has been read
+            if (j == 0 && items > 0 && !wait(&sh.o_free[t], (items - 1) & 1)) break;
+            if (!wait(&sh.p_full[t], (steps + j) & 1)) break;
+            tc_fence_after();
+            const uint64_t vd = smem_desc_mn_sw128(kv_addr + v.slot * L::TILE_BYTES, L::BLOCK_BYTES);
 #pragma unroll
-        for (int k = 0; k < BN / 16; ++k)
-          mma_f16_ta(t_o, t_s + k * 8, smem_desc_at(vd, k * 2048), IDESC_PV, j != 0 || k != 0);
-        mma_commit(&sh.o_full[t]);
-        mma_commit(&sh.empty[r.slot]);
-        return true;
-      };
-      Ring base{0, 0};  // of the step's first load
-      bool ok = full(base.at(k_load(t, 0))) && wait(&sh.q_full[SPLIT ? 0 : t], 0) && my_turn(0);
-      if (ok) {
-        tc_fence_after();
-        qk(base.at(k_load(t, 0)));
-        pass_turn();
+            for (int c = 0; c < BN / 16; ++c)
+              mma_f16_ta(t_o, t_s + c * 8, smem_desc_at(vd, c * 2048), IDESC_PV, j != 0 || c != 0);
+            if (more) {
+              qk(k);
+            } else {
+              mma_commit(&sh.o_full[t]);
+              pass_turn();
+            }
+            base = next;
+          }
+          steps += it.steps;
+          ++items;
+        }
+        mma_commit(&sh.drain[t]);
+        mbar_wait(&sh.drain[t], 0, kErrWaitTimeoutDrain);
       }
-      for (int j = 0; ok && j < steps; ++j) {
-        const Ring next = base.at(SPLIT ? 4 : 2);
-        const bool more = j + 1 < steps;
-        ok = full(base.at(v_load(t, 0))) && (!more || full(next.at(k_load(t, 0)))) && pv(base.at(v_load(t, 0)), j);
-        if (ok && more) qk(next.at(k_load(t, 0)));
-        pass_turn();
-        base = next;
-      }
-      if (!ok) sh.abort = 1;
-      mma_commit(&sh.drain[t]);
-      mbar_wait(&sh.drain[t], 0, kErrWaitTimeoutDrain);
     }
     __syncwarp();
-  }
   } else {
-    regs_inc<REGS_SOFTMAX>();
-    if ((warp >> 3) < tiles) {
     // ------------------------------------------------------------ softmax of half a row, output
+    regs_inc<REGS_SOFTMAX>();
     const int t = warp >> 3;
     const int half = (warp >> 2) & 1;  // of the keys of a tile, of the columns of O
     const int quarter = warp & 3;
@@ -399,193 +454,233 @@ tile_kernel(const __grid_constant__ CUtensorMap tq, const __grid_constant__ CUte
     auto wait = [&](uint64_t* bar, uint32_t parity) {
       good = __all_sync(0xffffffffu, mbar_wait_abort(bar, parity, kErrWaitTimeoutEpilogue, &sh.abort)) != 0 && good;
     };
-    float m = -INFINITY;
-    float2 l2 = make_float2(0.0f, 0.0f);
-    for (int j = 0; j < steps; ++j) {
-      const int64_t key0 = static_cast<int64_t>(key_tile(t, j)) * BN;
-      const float4* bias4 = BIAS ? reinterpret_cast<const float4*>(p.keys.bias + b * p.keys.bias_pitch + key0 + 64 * half) : nullptr;
-      const int64_t left64 = keys - key0;
-      const int left = left64 < BN ? static_cast<int>(left64) : BN;  // keys of this tile up to the last one
-      // one bit per key of this half that takes part (with a bias: per key up to the last one)
-      uint32_t bits[2] = {0xffffffffu, 0xffffffffu};
-      bool used = row < left;  // the key of this row's number
-      if (left < BN) {
-#pragma unroll
-        for (int w = 0; w < 2; ++w) {
-          const int n = left - 64 * half - 32 * w;
-          bits[w] = n >= 32 ? 0xffffffffu : n <= 0 ? 0u : (1u << n) - 1u;
-        }
+    uint32_t step0 = 0;   // steps of this tile before the item
+    uint32_t loads0 = 0;  // loads of both tiles before the item
+    uint32_t items0 = 0;  // items of this tile before the item
+#pragma unroll 1
+    for (int index = blockIdx.x; index < p.items; index += gridDim.x) {
+      const Item it = item_at<BIAS, SPLIT>(p, index);
+      const int b = it.b;
+      if (t >= it.tiles) {
+        loads0 += STEP_LOADS * it.steps;
+        continue;
       }
-      if (BIAS) {
-        used = used && __ldg(p.keys.bias + b * p.keys.bias_pitch + key0 + row) != -INFINITY;
-      } else if (p.keys.mask != nullptr) {
-        const uint8_t* mask = p.keys.mask + b * p.keys.mask_b;
-        used = used && __ldg(mask + (key0 + row) * p.keys.mask_k) != 0;
+      // One lane of a tile hands loads back to the producer: a tcgen05.commit holds the tensor cores up for
+      // about 120 cycles, so there is one a step (S_j ready) instead of one per thing that is done with.
+      const bool relay = quarter == 0 && half == 0 && lane == 0;
+      auto release = [&](uint32_t i) {
+        mbar_arrive(&sh.empty[i % L::STAGES]);
+        if (it.tiles == 1) mbar_arrive(&sh.empty[i % L::STAGES]);
+      };
+      float m = -INFINITY;
+      float2 l2 = make_float2(0.0f, 0.0f);
+#pragma unroll 1
+      for (int j = 0; j < it.steps; ++j) {
+        const int64_t key0 = static_cast<int64_t>(SPLIT ? it.j0 + 2 * j + t : j) * BN;
+        const float4* bias4 =
+            BIAS ? reinterpret_cast<const float4*>(p.keys.bias + b * p.keys.bias_pitch + key0 + 64 * half) : nullptr;
+        const int64_t left64 = it.keys - key0;
+        const int left = left64 < BN ? static_cast<int>(left64) : BN;  // keys of this tile up to the last one
+        // one bit per key of this half that takes part (with a bias: per key up to the last one)
+        uint32_t bits[2] = {0xffffffffu, 0xffffffffu};
+        bool used = row < left;  // the key of this row's number
+        if (left < BN) {
 #pragma unroll
-        for (int w = 0; w < 2; ++w) {
-          const int i = 64 * half + 32 * w + lane;
-          bits[w] = __ballot_sync(0xffffffffu, i < left && __ldg(mask + (key0 + i) * p.keys.mask_k) != 0);
+          for (int w = 0; w < 2; ++w) {
+            const int n = left - 64 * half - 32 * w;
+            bits[w] = n >= 32 ? 0xffffffffu : n <= 0 ? 0u : (1u << n) - 1u;
+          }
         }
-      }
-      const bool clear = !used && key0 + row < p.kv_len;
-      if (__any_sync(0xffffffffu, clear)) {
-        // wide: both tiles clear the same rows, each before its own second product
-        const int i = v_load(t, j);
-        wait(&sh.full[i % L::STAGES], (i / L::STAGES) & 1);
-        if (clear && good) {
-          uint4* v = reinterpret_cast<uint4*>(sKV + (i % L::STAGES) * L::TILE_BYTES + row * 128 +
-                                              half * (DP == 128 ? L::BLOCK_BYTES : 64));
-#pragma unroll
-          for (int e = 0; e < DP / 16; ++e) v[e] = make_uint4(0, 0, 0, 0);
-        }
-        fence_proxy_async_smem();
-      }
-      wait(&sh.s_full[t], j & 1);
-      tc_fence_after();
-      if (live) {
-        uint32_t r[64];
-        tmem_ld_32x32b_x32(t_s + 64 * half, *reinterpret_cast<uint32_t(*)[32]>(r));
-        tmem_ld_32x32b_x32(t_s + 64 * half + 32, *reinterpret_cast<uint32_t(*)[32]>(r + 32));
-        tmem_ld_wait();
-        reg_dep32(*reinterpret_cast<uint32_t(*)[32]>(r));
-        reg_dep32(*reinterpret_cast<uint32_t(*)[32]>(r + 32));
-        float* y = reinterpret_cast<float*>(r);
         if (BIAS) {
+          used = used && __ldg(p.keys.bias + b * p.keys.bias_pitch + key0 + row) != -INFINITY;
+        } else if (p.keys.mask != nullptr) {
+          const uint8_t* mask = p.keys.mask + b * p.keys.mask_b;
+          used = used && __ldg(mask + (key0 + row) * p.keys.mask_k) != 0;
 #pragma unroll
-          for (int e = 0; e < 64; e += 4) {
-            // an excluded key's score may be NaN; behind the last key the bias row may have ended
-            const float4 a = (bits[e / 32] >> (e & 31)) & 1 ? __ldg(bias4 + e / 4)
-                                                            : make_float4(-INFINITY, -INFINITY, -INFINITY, -INFINITY);
-            y[e + 0] = a.x == -INFINITY ? -INFINITY : fmaf(y[e + 0], scale2, a.x);
-            y[e + 1] = a.y == -INFINITY ? -INFINITY : fmaf(y[e + 1], scale2, a.y);
-            y[e + 2] = a.z == -INFINITY ? -INFINITY : fmaf(y[e + 2], scale2, a.z);
-            y[e + 3] = a.w == -INFINITY ? -INFINITY : fmaf(y[e + 3], scale2, a.w);
+          for (int w = 0; w < 2; ++w) {
+            const int i = 64 * half + 32 * w + lane;
+            bits[w] = __ballot_sync(0xffffffffu, i < left && __ldg(mask + (key0 + i) * p.keys.mask_k) != 0);
           }
-        } else if ((bits[0] & bits[1]) != 0xffffffffu) {
-#pragma unroll
-          for (int e = 0; e < 64; ++e) y[e] = (bits[e / 32] >> (e & 31)) & 1 ? y[e] : -INFINITY;
         }
-        float mx[4] = {y[0], y[1], y[2], y[3]};
+        const bool clear = !used && key0 + row < p.kv_len;
+        if (__any_sync(0xffffffffu, clear)) {
+          // wide: both tiles clear the same rows, each before its own second product
+          const uint32_t i = loads0 + STEP_LOADS * j + v_load(t), slot = i % L::STAGES;
+          wait(&sh.full[slot], (i / L::STAGES) & 1);
+          if (clear && good) {
+            uint4* v = reinterpret_cast<uint4*>(sKV + slot * L::TILE_BYTES + row * 128 +
+                                                half * (DP == 128 ? L::BLOCK_BYTES : 64));
 #pragma unroll
-        for (int e = 4; e < 60; e += 8) {
-#pragma unroll
-          for (int u = 0; u < 4; ++u) mx[u] = fmax3(mx[u], y[e + u], y[e + 4 + u]);
+            for (int e = 0; e < DP / 16; ++e) v[e] = make_uint4(0, 0, 0, 0);
+          }
+          fence_proxy_async_smem();
         }
+        wait(&sh.s_full[t], (step0 + j) & 1);
+        tc_fence_after();
+        // S_j is there, so Q K_j and before it P_{j-1} V_{j-1} are done (one thread issued them in order)
+        if (relay) {
+          release(loads0 + STEP_LOADS * j + k_load(t));
+          if (j > 0) release(loads0 + STEP_LOADS * (j - 1) + v_load(t));
+          if (j + 1 == it.steps) mbar_arrive(&sh.q_free[SPLIT ? 0 : t]);
+        }
+        if (live) {
+          uint32_t r[64];
+          tmem_ld_32x32b_x32(t_s + 64 * half, *reinterpret_cast<uint32_t(*)[32]>(r));
+          tmem_ld_32x32b_x32(t_s + 64 * half + 32, *reinterpret_cast<uint32_t(*)[32]>(r + 32));
+          tmem_ld_wait();
+          reg_dep32(*reinterpret_cast<uint32_t(*)[32]>(r));
+          reg_dep32(*reinterpret_cast<uint32_t(*)[32]>(r + 32));
+          float* y = reinterpret_cast<float*>(r);
+          if (BIAS) {
 #pragma unroll
-        for (int u = 0; u < 4; ++u) mx[u] = fmaxf(mx[u], y[60 + u]);
-        float top = fmaxf(fmax3(mx[0], mx[1], mx[2]), mx[3]);
-        // the other half's maximum (it is read before that half's arrival at p_full, so the next step's
-        // value cannot overtake it); the barrier also lets a half write its weights over the scores that
-        // the other has read by now
-        sh.x[t][half][row] = top;
-        named_barrier(3 + 4 * t + quarter, 64);
-        top = fmaxf(top, sh.x[t][half ^ 1][row]);
-        const float m_new = fmaxf(m, BIAS ? top : top * scale2);
-        if (j == 0) {
-          m = m_new;
-        } else if (__any_sync(0xffffffffu, real && m_new > m + GROWTH)) {
-          const float alpha = m_new == -INFINITY ? 1.0f : ex2_approx(m - m_new);
-          m = m_new;
-          l2 = mul2(l2, make_float2(alpha, alpha));
-          wait(&sh.o_full[t], (j - 1) & 1);
-          tc_fence_after();
+            for (int e = 0; e < 64; e += 4) {
+              // an excluded key's score may be NaN; behind the last key the bias row may have ended
+              const float4 a = (bits[e / 32] >> (e & 31)) & 1 ? __ldg(bias4 + e / 4)
+                                                              : make_float4(-INFINITY, -INFINITY, -INFINITY, -INFINITY);
+              y[e + 0] = a.x == -INFINITY ? -INFINITY : fmaf(y[e + 0], scale2, a.x);
+              y[e + 1] = a.y == -INFINITY ? -INFINITY : fmaf(y[e + 1], scale2, a.y);
+              y[e + 2] = a.z == -INFINITY ? -INFINITY : fmaf(y[e + 2], scale2, a.z);
+              y[e + 3] = a.w == -INFINITY ? -INFINITY : fmaf(y[e + 3], scale2, a.w);
+            }
+          } else if ((bits[0] & bits[1]) != 0xffffffffu) {
+#pragma unroll
+            for (int e = 0; e < 64; ++e) y[e] = (bits[e / 32] >> (e & 31)) & 1 ? y[e] : -INFINITY;
+          }
+          float mx[4] = {y[0], y[1], y[2], y[3]};
+#pragma unroll
+          for (int e = 4; e < 60; e += 8) {
+#pragma unroll
+            for (int u = 0; u < 4; ++u) mx[u] = fmax3(mx[u], y[e + u], y[e + 4 + u]);
+          }
+#pragma unroll
+          for (int u = 0; u < 4; ++u) mx[u] = fmaxf(mx[u], y[60 + u]);
+          float top = fmaxf(fmax3(mx[0], mx[1], mx[2]), mx[3]);
+          // the other half's maximum (it is read before that half's arrival at p_full, so the next step's
+          // value cannot overtake it); the barrier also lets a half write its weights over the scores that
+          // the other has read by now
+          sh.x[t][half][row] = top;
+          named_barrier(1 + 4 * t + quarter, 64);
+          top = fmaxf(top, sh.x[t][half ^ 1][row]);
+          const float m_new = fmaxf(m, BIAS ? top : top * scale2);
+          if (j == 0) {
+            m = m_new;
+          } else if (__any_sync(0xffffffffu, real && m_new > m + GROWTH)) {
+            const float alpha = m_new == -INFINITY ? 1.0f : ex2_approx(m - m_new);
+            m = m_new;
+            l2 = mul2(l2, make_float2(alpha, alpha));
 #pragma unroll 1
-          for (int c = 0; c < DP / 2; c += 16) {
-            uint32_t o[16];
-            tmem_ld_32x32b_x16(t_o + c, o);
-            tmem_ld_wait();
-            reg_dep16(o);
+            for (int c = 0; c < DP / 2; c += 16) {
+              uint32_t o[16];
+              tmem_ld_32x32b_x16(t_o + c, o);
+              tmem_ld_wait();
+              reg_dep16(o);
 #pragma unroll
-            for (int e = 0; e < 16; ++e) o[e] = __float_as_uint(__uint_as_float(o[e]) * alpha);
-            tmem_st_32x32b_x16(t_o + c, o);
+              for (int e = 0; e < 16; ++e) o[e] = __float_as_uint(__uint_as_float(o[e]) * alpha);
+              tmem_st_32x32b_x16(t_o + c, o);
+            }
           }
-        }
-        const float off = m == -INFINITY ? 0.0f : -m;
-        const float sc = BIAS ? 1.0f : scale2;
-        const float2 off2 = make_float2(off, off), sc2 = make_float2(sc, sc);
+          const float off = m == -INFINITY ? 0.0f : -m;
+          const float sc = BIAS ? 1.0f : scale2;
+          const float2 off2 = make_float2(off, off), sc2 = make_float2(sc, sc);
 #pragma unroll
-        for (int c = 0; c < 64; c += 32) {
-          uint32_t w[16];
-          weights<T>(y + c, sc2, off2, l2, w);
-          tmem_st_32x32b_x16(t_s + 32 * half + c / 2, w);
+          for (int c = 0; c < 64; c += 32) {
+            uint32_t w[16];
+            weights<T>(y + c, sc2, off2, l2, w);
+            tmem_st_32x32b_x16(t_s + 32 * half + c / 2, w);
+          }
+          tmem_st_wait();
         }
-        tmem_st_wait();
+        tc_fence_before();
+        __syncwarp();
+        if (lane == 0) mbar_arrive(&sh.p_full[t]);
       }
-      tc_fence_before();
-      __syncwarp();
-      if (lane == 0) mbar_arrive(&sh.p_full[t]);
-    }
-    if (steps > 0) {
-      wait(&sh.o_full[t], (steps - 1) & 1);
-      tc_fence_after();
-    }
-    // the sum over both halves
-    sh.x[t][half][row] = l2.x + l2.y;
-    named_barrier(3 + 4 * t + quarter, 64);
-    const float l = sh.x[t][0][row] + sh.x[t][1][row];
-    if (SPLIT) {
-      // (m, l) and O of this piece; O stays unwritten where no key took part
-      if (good && !sh.abort && live) {
-        const int64_t items = static_cast<int64_t>(gridDim.x / p.splits) * gridDim.y * gridDim.z;
-        const int64_t item = (static_cast<int64_t>(b) * gridDim.y + hk) * (gridDim.x / p.splits) + q_tile;
-        const int64_t at = ((2 * split + t) * items + item) * p.rows + row;
-        const int64_t parts = 2 * p.splits;
-        const bool exists = row < p.rows;
-        if (exists && half == 0) reinterpret_cast<float2*>(p.partial)[at] = make_float2(m, l);
-        if (steps > 0) {
-          float* o = p.partial + 2 * parts * items * p.rows + at * DP + half * (DP / 2);
+      if (it.steps > 0) {
+        wait(&sh.o_full[t], items0 & 1);
+        tc_fence_after();
+        if (relay) release(loads0 + STEP_LOADS * (it.steps - 1) + v_load(t));
+        ++items0;
+      }
+      // the sum over both halves
+      sh.x[t][half][row] = l2.x + l2.y;
+      named_barrier(1 + 4 * t + quarter, 64);
+      const float l = sh.x[t][0][row] + sh.x[t][1][row];
+      named_barrier(1 + 4 * t + quarter, 64);  // both have read it before the next item's maxima
+      if (SPLIT) {
+        // (m, l) and O of this piece; O stays unwritten where no key took part
+        if (good && live) {
+          const int64_t parts = 2 * p.splits, row_tiles = p.items / p.splits;
+          const int64_t at = ((2 * it.split + t) * row_tiles + index / p.splits) * p.rows + row;
+          const bool exists = row < p.rows;
+          if (exists && half == 0) reinterpret_cast<float2*>(p.partial)[at] = make_float2(m, l);
+          if (it.steps > 0) {
+            float* o = p.partial + 2 * parts * row_tiles * p.rows + at * DP + half * (DP / 2);
 #pragma unroll 1
-          for (int c = 0; c < DP / 2; c += 32) {
-            uint32_t r[32];
-            tmem_ld_32x32b_x32(t_o + c, r);
-            tmem_ld_wait();
-            reg_dep32(r);
-            if (exists) {
+            for (int c = 0; c < DP / 2; c += 32) {
+              uint32_t r[32];
+              tmem_ld_32x32b_x32(t_o + c, r);
+              tmem_ld_wait();
+              reg_dep32(r);
+              if (exists) {
 #pragma unroll
-              for (int u = 0; u < 8; ++u)
-                reinterpret_cast<uint4*>(o + c)[u] = make_uint4(r[4 * u], r[4 * u + 1], r[4 * u + 2], r[4 * u + 3]);
+                for (int u = 0; u < 8; ++u)
+                  reinterpret_cast<uint4*>(o + c)[u] = make_uint4(r[4 * u], r[4 * u + 1], r[4 * u + 2], r[4 * u + 3]);
+              }
             }
           }
         }
-      }
-    } else {
-      // the tile's rows leave through the shared memory of its queries
-      uint8_t* stage = sQ + t * L::TILE_BYTES;
-      if (good) {
+        if (it.steps > 0) {
+          tc_fence_before();
+          __syncwarp();
+          if (lane == 0) mbar_arrive(&sh.o_free[t]);
+        }
+      } else {
+        // 32 columns of the warp's 32 rows at a time through its own shared memory (16-byte chunk u of row
+        // r at u ^ (r >> 1 & 3)), then 64-byte pieces of 8 rows a store
         const float inv = l == 0.0f ? 0.0f : 1.0f / l;
+        uint8_t* stage = smem + L::OFF_STAGING + warp * L::STAGING_BYTES;
 #pragma unroll 1
         for (int c = 0; c < DP / 2; c += 32) {
           uint32_t r[32];
-          if (steps > 0) {
+          if (it.steps > 0) {
             tmem_ld_32x32b_x32(t_o + c, r);
             tmem_ld_wait();
             reg_dep32(r);
+            if (c + 32 == DP / 2) {
+              tc_fence_before();
+              __syncwarp();
+              if (lane == 0) mbar_arrive(&sh.o_free[t]);
+            }
           } else {
 #pragma unroll
             for (int e = 0; e < 32; ++e) r[e] = 0;
           }
-          const int col = half * (DP / 2) + c;
-          uint8_t* dst = stage + (col >> 6) * L::BLOCK_BYTES + row * 128;
+          __syncwarp();
 #pragma unroll
           for (int u = 0; u < 4; ++u) {
             uint32_t w[4];
 #pragma unroll
             for (int e = 0; e < 4; ++e)
               w[e] = pack2<T>(__uint_as_float(r[8 * u + 2 * e]) * inv, __uint_as_float(r[8 * u + 2 * e + 1]) * inv);
-            const int chunk = ((col & 63) >> 3) + u;
-            *reinterpret_cast<uint4*>(dst + ((chunk ^ (row & 7)) << 4)) = make_uint4(w[0], w[1], w[2], w[3]);
+            *reinterpret_cast<uint4*>(stage + lane * 64 + ((u ^ (lane >> 1 & 3)) << 4)) = make_uint4(w[0], w[1], w[2], w[3]);
+          }
+          __syncwarp();
+          const int chunk = lane & 3, col = half * (DP / 2) + c + chunk * 8;
+          if (good && col < p.dim) {
+#pragma unroll
+            for (int i = 0; i < 4; ++i) {
+              const int sr = i * 8 + (lane >> 2), tr = quarter * 32 + sr;
+              const int tok = tr / p.group, h = it.hk * p.group + tr - tok * p.group;
+              const int64_t token = it.tok0 + t * p.tokens + tok;
+              if (tok < p.tokens && token < p.q_len)
+                *reinterpret_cast<uint4*>(static_cast<T*>(p.out.data) + b * p.out.stride_b + token * p.out.stride_s +
+                                          h * p.out.stride_h + col) =
+                    *reinterpret_cast<const uint4*>(stage + sr * 64 + ((chunk ^ (sr >> 1 & 3)) << 4));
+            }
           }
         }
-        fence_proxy_async_smem();
       }
-      named_barrier(1 + t, 2 * BM);  // reached on every path
-      if (good && !sh.abort && quarter == 0 && half == 0 && lane == 0) {
-        for (int c = 0; c < L::BLOCKS; ++c)
-          tma_store_4d(&to, stage + c * L::BLOCK_BYTES, c * 64, hk * p.group, static_cast<int32_t>(tok0 + t * p.tokens), b);
-        bulk_commit_group();
-        bulk_wait_group<0>();
-      }
-    }
+      step0 += it.steps;
+      loads0 += STEP_LOADS * it.steps;
     }
   }
   tc_fence_before();
@@ -680,8 +775,8 @@ struct Plan {
 
 // The wide form takes 2 row tiles x 1 key tile a step, SPLIT 1 row tile x 2 key tiles, which moves twice
 // the keys and values through L2 for the same work (a step takes 1.35 times as long at 16384 x 16111 x
-// 24 heads of 128). Costs in wide steps (about 2.2 us): a wave of CTAs has to start and end (2), joining
-// costs 1.5. The cheapest wins: few rows are split, many waves of CTAs are not.
+// 24 heads of 128). Costs in wide steps (about 2 us): an item's ends cost 0.7, a launch 2, joining the
+// pieces 1.5. The cheapest wins: few rows are split, many waves of items are not.
 inline Plan make_plan(int64_t batch, int64_t q_len, int64_t kv_len, int heads, int kv_heads, int dim) {
   Plan p{};
   p.group = heads / kv_heads;
@@ -689,11 +784,11 @@ inline Plan make_plan(int64_t batch, int64_t q_len, int64_t kv_len, int heads, i
   p.q_tiles = (q_len + p.tokens - 1) / p.tokens;
   const int64_t nk = (kv_len + BN - 1) / BN, base = batch * kv_heads, sms = sm_count();
   auto waves = [&](int64_t ctas) { return (ctas + sms - 1) / sms; };
-  double best = static_cast<double>(waves(base * ((p.q_tiles + 1) / 2))) * (2.0 + static_cast<double>(nk));
+  double best = static_cast<double>(waves(base * ((p.q_tiles + 1) / 2))) * (0.7 + static_cast<double>(nk)) + 2.0;
   for (int64_t s = 1; s <= 64 && 2 * (s - 1) < nk; ++s) {
     const int64_t per = (nk + 2 * s - 1) / (2 * s) * 2;
     if ((s - 1) * per >= nk) continue;  // the last CTAs would have nothing
-    const double cost = static_cast<double>(waves(base * p.q_tiles * s)) * (2.0 + 1.35 * static_cast<double>(per) / 2) + 1.5;
+    const double cost = static_cast<double>(waves(base * p.q_tiles * s)) * (0.7 + 1.35 * static_cast<double>(per) / 2) + 3.5;
     if (cost < best && base * p.q_tiles * s < (int64_t{1} << 24)) {
       best = cost;
       p.splits = static_cast<int>(s);
@@ -710,11 +805,10 @@ inline Plan make_plan(int64_t batch, int64_t q_len, int64_t kv_len, int heads, i
 template <typename T, int DP, bool BIAS, bool SPLIT>
 cudaError_t launch(const Params& p, const Plan& plan, cudaStream_t st) {
   constexpr bool BF16 = std::is_same<T, __nv_bfloat16>::value;
-  CUtensorMap mq, mk, mv, mo;
+  CUtensorMap mq, mk, mv;
   // without keys k and v may be null: their maps are never used
   const bool any = p.kv_len > 0;
   if (!make_map(&mq, BF16, p.q, p.batch, p.q_len, p.heads, p.dim, plan.group, plan.tokens) ||
-      !make_map(&mo, BF16, p.out, p.batch, p.q_len, p.heads, p.dim, plan.group, plan.tokens) ||
       !make_map(&mk, BF16, any ? p.k : p.q, p.batch, any ? p.kv_len : 1, any ? p.kv_heads : 1, p.dim, 1, BN) ||
       !make_map(&mv, BF16, any ? p.v : p.q, p.batch, any ? p.kv_len : 1, any ? p.kv_heads : 1, p.dim, 1, BN))
     return cudaErrorInvalidValue;
@@ -731,18 +825,20 @@ cudaError_t launch(const Params& p, const Plan& plan, cudaStream_t st) {
                                 static_cast<int>(smem));
   });
   if (e != cudaSuccess) return e;
-  const TileParams tp{p.q_len, p.kv_len, plan.group, plan.tokens, p.k.stride_b != 0, p.k.stride_h != 0,
-                      p.v.stride_b != 0, p.v.stride_h != 0, p.scale2, p.keys, plan.splits, plan.per, plan.rows, p.partial};
-  const int64_t x = SPLIT ? plan.q_tiles * plan.splits : (plan.q_tiles + 1) / 2;
-  const dim3 grid(static_cast<unsigned>(x), static_cast<unsigned>(p.kv_heads), static_cast<unsigned>(p.batch));
-  tile_kernel<T, DP, BIAS, SPLIT><<<grid, THREADS, smem, st>>>(mq, mk, mv, mo, tp);
+  const int64_t per_head = SPLIT ? plan.q_tiles * plan.splits : (plan.q_tiles + 1) / 2;
+  const int64_t items = per_head * p.kv_heads * p.batch;
+  TileParams tp{p.out, p.q_len, p.kv_len, p.kv_heads, p.dim, plan.group, plan.tokens, p.k.stride_b != 0,
+                p.k.stride_h != 0, p.v.stride_b != 0, p.v.stride_h != 0, p.scale2, p.keys, static_cast<int>(items),
+                static_cast<int>(per_head), plan.splits, plan.per, plan.rows, p.partial};
+  const int64_t sms = sm_count();
+  tile_kernel<T, DP, BIAS, SPLIT><<<static_cast<unsigned>(items < sms ? items : sms), THREADS, smem, st>>>(mq, mk, mv, tp);
   if ((e = cudaGetLastError()) != cudaSuccess) return e;
   note_launch();
   if (SPLIT) {
-    const int64_t items = p.batch * p.kv_heads * plan.q_tiles;
-    split_kernel<T, DP><<<static_cast<unsigned>(items * plan.rows), 256, 0, st>>>(
+    const int64_t tiles = items / plan.splits;
+    split_kernel<T, DP><<<static_cast<unsigned>(tiles * plan.rows), 256, 0, st>>>(
         p.partial, p.out, p.q_len, plan.group, plan.tokens, plan.rows, static_cast<int>(plan.q_tiles), p.kv_heads,
-        2 * plan.splits, items, p.dim);
+        2 * plan.splits, tiles, p.dim);
     if ((e = cudaGetLastError()) != cudaSuccess) return e;
     note_launch();
   }
@@ -782,7 +878,9 @@ static int checks(int64_t batch, int64_t q_len, int64_t kv_len, int heads, int k
     return fail(SLIM_ERR_SHAPE, "head dim must be a multiple of 8 up to %d, got %d", MAX_DIM, dim);
   if (heads % kv_heads || heads / kv_heads > 128)
     return fail(SLIM_ERR_SHAPE, "%d query heads do not group over %d key heads (at most 128 each)", heads, kv_heads);
-  if (batch >= (int64_t{1} << 16) || q_len >= (int64_t{1} << 31) - 256 || kv_len >= (int64_t{1} << 31) - 256 || heads >= (1 << 16))
+  const int64_t tokens = 128 / (heads / kv_heads);
+  if (batch >= (int64_t{1} << 16) || q_len >= (int64_t{1} << 31) - 256 || kv_len >= (int64_t{1} << 31) - 256 || heads >= (1 << 16) ||
+      (q_len + tokens - 1) / tokens * kv_heads * (batch < 1 ? 1 : batch) >= (int64_t{1} << 31))
     return fail(SLIM_ERR_SHAPE, "attention shape too large");
   return SLIM_OK;
 }

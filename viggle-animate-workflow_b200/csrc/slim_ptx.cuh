@@ -95,6 +95,18 @@ __device__ __forceinline__ bool mbar_wait(uint64_t* bar, uint32_t parity, unsign
   }
 }
 
+__device__ __forceinline__ bool mbar_test_wait(uint64_t* bar, uint32_t parity) {
+  uint32_t ok;
+  asm volatile(
+      "{\n\t.reg .pred p;\n\t"
+      "mbarrier.test_wait.parity.shared::cta.b64 p, [%1], %2;\n\t"
+      "selp.u32 %0, 1, 0, p;\n\t}"
+      : "=r"(ok)
+      : "r"(smem_u32(bar)), "r"(parity)
+      : "memory");
+  return ok != 0;
+}
+
 // The same, giving up as well (without a code of its own) once another warp has set *abort.
 __device__ __forceinline__ bool mbar_wait_abort(uint64_t* bar, uint32_t parity, unsigned int code, volatile int* abort) {
   if (mbar_try_wait(bar, parity)) return true;
@@ -108,6 +120,14 @@ __device__ __forceinline__ bool mbar_wait_abort(uint64_t* bar, uint32_t parity, 
       return false;
     }
   }
+}
+
+// mbar_wait_abort that polls instead of suspending the thread (which takes some 200 cycles to come
+// back): for a single thread on whose reaction others wait.
+__device__ __forceinline__ bool mbar_poll_abort(uint64_t* bar, uint32_t parity, unsigned int code, volatile int* abort) {
+  for (int i = 0; i < 256; ++i)
+    if (mbar_test_wait(bar, parity)) return true;
+  return mbar_wait_abort(bar, parity, code, abort);
 }
 
 // ---------------------------------------------------------------- TMA (no multicast)
