@@ -130,7 +130,7 @@ __global__ void __launch_bounds__(1024) bias_kernel(const void* __restrict__ mas
 // rows of V are cleared in shared memory, as 0 * NaN is not 0.
 namespace tile {
 constexpr int BM = 128, BN = KEY_TILE;
-constexpr int SOFTMAX_WARPS = 16, WARP_TMA = 16, WARP_MMA = 17;
+constexpr int SOFTMAX_WARPS = 16, WARP_TMA = 16, WARP_MMA = 17, WARP_RELAY = 19;
 constexpr int WARPS = 20, THREADS = 32 * WARPS;
 // Registers: 96 a thread at launch, of which the softmax warps take 104 and the last warpgroup leaves
 // all but 64: 4 x 104 + 64 = 5 x 96.
@@ -242,6 +242,18 @@ __device__ __forceinline__ void weights(const float* y, float2 sc2, float2 off2,
     l2 = add2(l2, g);
     w[e] = pack2<T>(g.x, g.y);
   }
+}
+
+__device__ __forceinline__ float row_max(const float* y) {
+  float mx[4] = {y[0], y[1], y[2], y[3]};
+#pragma unroll
+  for (int e = 4; e < 60; e += 8) {
+#pragma unroll
+    for (int u = 0; u < 4; ++u) mx[u] = fmax3(mx[u], y[e + u], y[e + 4 + u]);
+  }
+#pragma unroll
+  for (int u = 0; u < 4; ++u) mx[u] = fmaxf(mx[u], y[60 + u]);
+  return fmaxf(fmax3(mx[0], mx[1], mx[2]), mx[3]);
 }
 
 template <typename T, int DP, bool BIAS, bool SPLIT>
@@ -433,6 +445,38 @@ tile_kernel(const __grid_constant__ CUtensorMap tq, const __grid_constant__ CUte
         mbar_wait(&sh.drain[t], 0, kErrWaitTimeoutDrain);
       }
     }
+    else if (warp == WARP_RELAY && lane == 0) {
+      // ---------------------------------------------------------- tiles handed back to the producer
+      // A tcgen05.commit holds the tensor cores up for about 120 cycles, so there is one a step (S_j ready,
+      // hence Q K_j done, and before it P_{j-1} V_{j-1}: one thread issued them in order) instead of one
+      // for each tile of keys and values that is done with; this thread passes it on.
+      uint32_t loads = 0, steps[2] = {0, 0}, items[2] = {0, 0};
+      bool ok = true;
+      auto wait = [&](uint64_t* bar, uint32_t ph) {
+        ok = ok && mbar_wait_abort(bar, ph, kErrWaitTimeoutMma, &sh.abort);
+        return ok;
+      };
+      for (int index = blockIdx.x; ok && index < p.items; index += gridDim.x) {
+        const Item it = item_at<BIAS, SPLIT>(p, index);
+        auto release = [&](uint32_t i) {
+          mbar_arrive(&sh.empty[i % L::STAGES]);
+          if (it.tiles == 1) mbar_arrive(&sh.empty[i % L::STAGES]);
+        };
+        for (int j = 0; ok && j < it.steps; ++j) {
+          for (int t = 0; t < it.tiles && wait(&sh.s_full[t], (steps[t] + j) & 1); ++t) {
+            release(loads + STEP_LOADS * j + k_load(t));
+            if (j > 0) release(loads + STEP_LOADS * (j - 1) + v_load(t));
+            if (j + 1 == it.steps) mbar_arrive(&sh.q_free[SPLIT ? 0 : t]);
+          }
+        }
+        for (int t = 0; it.steps > 0 && t < it.tiles && wait(&sh.o_full[t], items[t] & 1); ++t) {
+          release(loads + STEP_LOADS * (it.steps - 1) + v_load(t));
+          steps[t] += it.steps;
+          ++items[t];
+        }
+        loads += STEP_LOADS * it.steps;
+      }
+    }
     __syncwarp();
   } else {
     // ------------------------------------------------------------ softmax of half a row, output
@@ -465,13 +509,6 @@ tile_kernel(const __grid_constant__ CUtensorMap tq, const __grid_constant__ CUte
         loads0 += STEP_LOADS * it.steps;
         continue;
       }
-      // One lane of a tile hands loads back to the producer: a tcgen05.commit holds the tensor cores up for
-      // about 120 cycles, so there is one a step (S_j ready) instead of one per thing that is done with.
-      const bool relay = quarter == 0 && half == 0 && lane == 0;
-      auto release = [&](uint32_t i) {
-        mbar_arrive(&sh.empty[i % L::STAGES]);
-        if (it.tiles == 1) mbar_arrive(&sh.empty[i % L::STAGES]);
-      };
       float m = -INFINITY;
       float2 l2 = make_float2(0.0f, 0.0f);
 #pragma unroll 1
@@ -517,12 +554,6 @@ tile_kernel(const __grid_constant__ CUtensorMap tq, const __grid_constant__ CUte
         }
         wait(&sh.s_full[t], (step0 + j) & 1);
         tc_fence_after();
-        // S_j is there, so Q K_j and before it P_{j-1} V_{j-1} are done (one thread issued them in order)
-        if (relay) {
-          release(loads0 + STEP_LOADS * j + k_load(t));
-          if (j > 0) release(loads0 + STEP_LOADS * (j - 1) + v_load(t));
-          if (j + 1 == it.steps) mbar_arrive(&sh.q_free[SPLIT ? 0 : t]);
-        }
         if (live) {
           uint32_t r[64];
           tmem_ld_32x32b_x32(t_s + 64 * half, *reinterpret_cast<uint32_t(*)[32]>(r));
@@ -546,48 +577,52 @@ tile_kernel(const __grid_constant__ CUtensorMap tq, const __grid_constant__ CUte
 #pragma unroll
             for (int e = 0; e < 64; ++e) y[e] = (bits[e / 32] >> (e & 31)) & 1 ? y[e] : -INFINITY;
           }
-          float mx[4] = {y[0], y[1], y[2], y[3]};
-#pragma unroll
-          for (int e = 4; e < 60; e += 8) {
-#pragma unroll
-            for (int u = 0; u < 4; ++u) mx[u] = fmax3(mx[u], y[e + u], y[e + 4 + u]);
-          }
-#pragma unroll
-          for (int u = 0; u < 4; ++u) mx[u] = fmaxf(mx[u], y[60 + u]);
-          float top = fmaxf(fmax3(mx[0], mx[1], mx[2]), mx[3]);
-          // the other half's maximum (it is read before that half's arrival at p_full, so the next step's
-          // value cannot overtake it); the barrier also lets a half write its weights over the scores that
-          // the other has read by now
-          sh.x[t][half][row] = top;
-          named_barrier(1 + 4 * t + quarter, 64);
-          top = fmaxf(top, sh.x[t][half ^ 1][row]);
-          const float m_new = fmaxf(m, BIAS ? top : top * scale2);
-          if (j == 0) {
-            m = m_new;
-          } else if (__any_sync(0xffffffffu, real && m_new > m + GROWTH)) {
-            const float alpha = m_new == -INFINITY ? 1.0f : ex2_approx(m - m_new);
-            m = m_new;
-            l2 = mul2(l2, make_float2(alpha, alpha));
-#pragma unroll 1
-            for (int c = 0; c < DP / 2; c += 16) {
-              uint32_t o[16];
-              tmem_ld_32x32b_x16(t_o + c, o);
-              tmem_ld_wait();
-              reg_dep16(o);
-#pragma unroll
-              for (int e = 0; e < 16; ++e) o[e] = __float_as_uint(__uint_as_float(o[e]) * alpha);
-              tmem_st_32x32b_x16(t_o + c, o);
-            }
-          }
-          const float off = m == -INFINITY ? 0.0f : -m;
+          // Weights 2^(y sc - m). From the second step on they are taken with the m in use, and only if some
+          // row's maximum then turns out to have grown too far are they taken again: that keeps the maxima
+          // off the way from the scores to the weights.
           const float sc = BIAS ? 1.0f : scale2;
-          const float2 off2 = make_float2(off, off), sc2 = make_float2(sc, sc);
+          const int pair = 1 + 4 * t + quarter;  // barrier of both halves
+          float2 add = make_float2(0.0f, 0.0f);
+          auto store_weights = [&] {
+            const float off = m == -INFINITY ? 0.0f : -m;
+            const float2 off2 = make_float2(off, off), sc2 = make_float2(sc, sc);
+            add = make_float2(0.0f, 0.0f);
 #pragma unroll
-          for (int c = 0; c < 64; c += 32) {
-            uint32_t w[16];
-            weights<T>(y + c, sc2, off2, l2, w);
-            tmem_st_32x32b_x16(t_s + 32 * half + c / 2, w);
+            for (int c = 0; c < 64; c += 32) {
+              uint32_t w[16];
+              weights<T>(y + c, sc2, off2, add, w);
+              tmem_st_32x32b_x16(t_s + 32 * half + c / 2, w);
+            }
+          };
+          if (j > 0) {
+            named_barrier(pair, 64);  // both halves have read the scores that the weights go over
+            store_weights();
           }
+          const float own = row_max(y) * sc;
+          if (j == 0 || named_barrier_any(pair, 64, real && own > m + GROWTH)) {
+            sh.x[t][half][row] = own;
+            named_barrier(pair, 64);
+            const float m_new = fmaxf(m, fmaxf(own, sh.x[t][half ^ 1][row]));
+            named_barrier(pair, 64);  // both have read it before it is written again
+            if (j > 0) {
+              // O holds P_0 V_0 + ... + P_{j-1} V_{j-1} (done before S_j)
+              const float alpha = m_new == -INFINITY ? 1.0f : ex2_approx(m - m_new);
+              l2 = mul2(l2, make_float2(alpha, alpha));
+#pragma unroll 1
+              for (int c = 0; c < DP / 2; c += 16) {
+                uint32_t o[16];
+                tmem_ld_32x32b_x16(t_o + c, o);
+                tmem_ld_wait();
+                reg_dep16(o);
+#pragma unroll
+                for (int e = 0; e < 16; ++e) o[e] = __float_as_uint(__uint_as_float(o[e]) * alpha);
+                tmem_st_32x32b_x16(t_o + c, o);
+              }
+            }
+            m = m_new;
+            store_weights();
+          }
+          l2 = add2(l2, add);
           tmem_st_wait();
         }
         tc_fence_before();
@@ -597,7 +632,6 @@ tile_kernel(const __grid_constant__ CUtensorMap tq, const __grid_constant__ CUte
       if (it.steps > 0) {
         wait(&sh.o_full[t], items0 & 1);
         tc_fence_after();
-        if (relay) release(loads0 + STEP_LOADS * (it.steps - 1) + v_load(t));
         ++items0;
       }
       // the sum over both halves

@@ -509,6 +509,20 @@ __device__ __forceinline__ void named_barrier(int id, int threads) {
   asm volatile("bar.sync %0, %1;" ::"r"(id), "r"(threads) : "memory");
 }
 
+// The same, returning whether `pred` holds in any of the threads.
+__device__ __forceinline__ bool named_barrier_any(int id, int threads, bool pred) {
+  uint32_t any;
+  asm volatile(
+      "{\n\t.reg .pred p, q;\n\t"
+      "setp.ne.u32 p, %3, 0;\n\t"
+      "barrier.cta.red.or.pred q, %1, %2, p;\n\t"
+      "selp.u32 %0, 1, 0, q;\n\t}"
+      : "=r"(any)
+      : "r"(id), "r"(threads), "r"(static_cast<uint32_t>(pred))
+      : "memory");
+  return any != 0;
+}
+
 // ---------------------------------------------------------------- packed fp32x2 (sm_100)
 // Each lane is an independent IEEE round-to-nearest fp32 operation, so a pair of values goes
 // through exactly the rounding steps of the scalar code.
