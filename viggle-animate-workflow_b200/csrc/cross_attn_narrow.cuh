@@ -211,8 +211,7 @@ narrow_kernel(const __grid_constant__ CUtensorMap tq, const __grid_constant__ CU
       const uint64_t v_desc = smem_desc_mn_sw128(smem_u32(sKV), Tile<DP>::BLOCK_BYTES);
       bool ok = true;
       auto wait = [&](uint64_t* bar, uint32_t ph) {
-        bool done = true;
-        if (lane == 0) done = mbar_poll_abort(bar, ph, kErrWaitTimeoutMma, &sh.abort);
+        const bool done = mbar_poll_abort(bar, ph, kErrWaitTimeoutMma, &sh.abort);
         ok = __all_sync(0xffffffffu, done) != 0 && ok;
         return ok;
       };
@@ -285,8 +284,7 @@ narrow_kernel(const __grid_constant__ CUtensorMap tq, const __grid_constant__ CU
     // once), so that a row's four warps meet at each of their barriers.
     bool good = true;
     auto wait = [&](uint64_t* bar, uint32_t parity) {
-      bool ok = true;
-      if (lane == 0) ok = mbar_wait_abort(bar, parity, kErrWaitTimeoutEpilogue, &sh.abort);
+      const bool ok = mbar_wait_abort(bar, parity, kErrWaitTimeoutEpilogue, &sh.abort);
       good = __all_sync(0xffffffffu, ok) != 0 && good;
     };
     // S_g, or (g beyond the last step) P_{g-2} V_{g-2} done

@@ -11,9 +11,9 @@ namespace wide {
 // of keys and values that is loaded. 20 warps:
 //   warps 0..7, 8..15  softmax of tile 0 / 1, half a row (64 keys) a thread: scores from TMEM, weights
 //                2^(s scale2 + bias - m) packed to 16 bits over the scores, where the second product reads
-//                them. From an item's second step on the weights are taken with the maximum in use; only if
-//                some row's maximum turns out to have grown by more than 2^8 over it are O and the sums
-//                rescaled and the weights taken again (weights stay below 2^8, sums and O are fp32).
+//                them. m is only changed, and O and the sums rescaled, when some row's maximum has grown by
+//                more than 2^8 over it (weights stay below 2^8, sums and O are fp32), which is rare after an
+//                item's first step.
 //   warp 16      TMA: queries, keys and values in the order of their use
 //   warp 17      the MMAs: S_t = Q_t K_0^T, then per step and tile O_t += P_t V_j followed at once by
 //                S_t = Q_t K_{j+1}^T: while one tile is in the softmax the tensor cores work on the other.
@@ -177,55 +177,65 @@ wide_kernel(const __grid_constant__ CUtensorMap tq, const __grid_constant__ CUte
       const uint64_t q_desc = smem_desc_sw128(smem_u32(sQ));
       const uint64_t k_desc = smem_desc_sw128(smem_u32(sKV) + L::TILE);
       const uint64_t v_desc = smem_desc_mn_sw128(smem_u32(sKV), Tile<DP>::BLOCK_BYTES);
-      uint32_t h = 0, steps[2] = {0, 0}, items[2] = {0, 0};  // steps in all, steps and items of each tile
+      // steps in all, and of each tile steps, items whose queries are in use, items whose output is begun
+      uint32_t h = 0, steps[2] = {0, 0}, q_items[2] = {0, 0}, o_items[2] = {0, 0};
       bool ok = true;
       auto wait = [&](uint64_t* bar, uint32_t ph) {
-        bool done = true;
-        if (lane == 0) done = mbar_poll_abort(bar, ph, kErrWaitTimeoutMma, &sh.abort);
+        const bool done = mbar_poll_abort(bar, ph, kErrWaitTimeoutMma, &sh.abort);
         ok = __all_sync(0xffffffffu, done) != 0 && ok;
         return ok;
       };
       auto full = [&](uint32_t n) { return wait(&sh.full[n % L::PAIRS], n / L::PAIRS & 1); };
       auto place = [](uint32_t n) { return n % L::PAIRS * (2 * L::TILE); };
-      for (int index = blockIdx.x; ok && index < p.items; index += gridDim.x) {
-        const Item it = item_at<BIAS>(p, index);
-        if (it.steps == 0) continue;
-        if (!full(h)) break;
-#pragma unroll
-        for (int t = 0; t < 2; ++t) {
-          if (t >= it.tiles || !wait(&sh.q_full[t], items[t] & 1)) break;
-          tc_fence_after();
-          if (leader) {
-            mma_scores<DP, BF16>(tm + col_s(t), smem_desc_at(q_desc, t * L::TILE), smem_desc_at(k_desc, place(h)));
-            mma_commit(&sh.s_full[t]);
-          }
-          __syncwarp();
+      auto next_item = [&](int index, Item& it) {  // the first one from index on that has keys
+        for (; index < p.items; index += gridDim.x) {
+          it = item_at<BIAS>(p, index);
+          if (it.steps > 0) break;
         }
+        return index;
+      };
+      // S_t = Q_t K^T of an item's first step, from place n
+      auto first_scores = [&](int t, uint32_t n) {
+        if (!wait(&sh.q_full[t], q_items[t]++ & 1)) return;
+        tc_fence_after();
+        if (leader) {
+          mma_scores<DP, BF16>(tm + col_s(t), smem_desc_at(q_desc, t * L::TILE), smem_desc_at(k_desc, place(n)));
+          mma_commit(&sh.s_full[t]);
+        }
+        __syncwarp();
+      };
+      Item it, next;
+      int index = next_item(blockIdx.x, it);
+      if (index < p.items && full(0)) {
+#pragma unroll
+        for (int t = 0; t < 2; ++t)
+          if (t < it.tiles) first_scores(t, 0);
+      }
+      while (ok && index < p.items) {
+        index = next_item(index + gridDim.x, next);
+        const int next_tiles = index < p.items ? next.tiles : 0;
         for (int j = 0; ok && j < it.steps; ++j, ++h) {
           const bool more = j + 1 < it.steps;
           if (!full(h + 1)) break;
 #pragma unroll
           for (int t = 0; t < 2; ++t) {
-            if (t >= it.tiles) break;
-            // the last item's output has been read
-            if (j == 0 && items[t] > 0 && !wait(&sh.o_free[t], (items[t] - 1) & 1)) break;
-            if (!wait(&sh.p_full[t], (steps[t] + j) & 1)) break;
-            tc_fence_after();
-            if (leader) {
-              mma_values<DP, BF16>(tm + col_o(t), tm + col_s(t), smem_desc_at(v_desc, place(h + 1)), j != 0);
-              if (more)
-                mma_scores<DP, BF16>(tm + col_s(t), smem_desc_at(q_desc, t * L::TILE), smem_desc_at(k_desc, place(h + 1)));
-              mma_commit(more ? &sh.s_full[t] : &sh.o_full[t]);
+            if (t < it.tiles) {
+              // the last item's output has been read
+              if (j == 0 && o_items[t]++ > 0 && !wait(&sh.o_free[t], o_items[t] & 1)) break;
+              if (!wait(&sh.p_full[t], steps[t]++ & 1)) break;
+              tc_fence_after();
+              if (leader) {
+                mma_values<DP, BF16>(tm + col_o(t), tm + col_s(t), smem_desc_at(v_desc, place(h + 1)), j != 0);
+                if (more)
+                  mma_scores<DP, BF16>(tm + col_s(t), smem_desc_at(q_desc, t * L::TILE), smem_desc_at(k_desc, place(h + 1)));
+                mma_commit(more ? &sh.s_full[t] : &sh.o_full[t]);
+              }
+              __syncwarp();
             }
-            __syncwarp();
+            if (!more && t < next_tiles) first_scores(t, h + 1);
           }
         }
-#pragma unroll
-        for (int t = 0; t < 2; ++t) {
-          if (t >= it.tiles) break;
-          steps[t] += it.steps;
-          ++items[t];
-        }
+        it = next;
       }
       if (leader) {
         mma_commit(&sh.drain);
@@ -274,8 +284,7 @@ wide_kernel(const __grid_constant__ CUtensorMap tq, const __grid_constant__ CUte
     // once), so that both halves meet at each of their barriers.
     bool good = true;
     auto wait = [&](uint64_t* bar, uint32_t parity) {
-      bool ok = true;
-      if (lane == 0) ok = mbar_wait_abort(bar, parity, kErrWaitTimeoutEpilogue, &sh.abort);
+      const bool ok = mbar_wait_abort(bar, parity, kErrWaitTimeoutEpilogue, &sh.abort);
       good = __all_sync(0xffffffffu, ok) != 0 && good;
       tc_fence_after();
     };
@@ -315,20 +324,8 @@ wide_kernel(const __grid_constant__ CUtensorMap tq, const __grid_constant__ CUte
         reg_dep32(*reinterpret_cast<uint32_t(*)[32]>(r + 32));
         float(&y)[64] = reinterpret_cast<float(&)[64]>(r);
         mask_scores<BIAS, 64>(p, it.b, key0, 64 * half, bits, y);
-        float2 add;
-        auto store_weights = [&] {
-          const float off = m == -INFINITY ? 0.0f : -m;
-          uint32_t w[16];
-          add = weights<T>(y, sc, off, w);
-          tmem_st_32x32b_x16(t_s + 32 * half, w);
-          add = add2(add, weights<T>(y + 32, sc, off, w));
-          tmem_st_32x32b_x16(t_s + 32 * half + 16, w);
-        };
-        if (j > 0) {
-          named_barrier(pair, 64);  // both halves have read the scores that the weights go over
-          store_weights();
-        }
         const float own = max_of<64>(y) * sc;
+        // (the barrier also tells that both halves have read the scores that the weights go over)
         if (j == 0 || named_barrier_any(pair, 64, real && own > m + GROWTH)) {
           const float m_new = fmaxf(m, fmaxf(own, other(own)));
           if (j > 0) {  // O holds P_0 V_0 + ... + P_{j-1} V_{j-1} (done before S_j)
@@ -337,9 +334,14 @@ wide_kernel(const __grid_constant__ CUtensorMap tq, const __grid_constant__ CUte
             rescale<DP / 2>(t_o, alpha);
           }
           m = m_new;
-          store_weights();
         }
-        l2 = add2(l2, add);
+        const float off = m == -INFINITY ? 0.0f : -m;
+#pragma unroll
+        for (int c = 0; c < 64; c += 32) {
+          uint32_t w[16];
+          l2 = add2(l2, weights<T>(y + c, sc, off, w));
+          tmem_st_32x32b_x16(t_s + 32 * half + c / 2, w);
+        }
         tmem_st_wait();
         if (__any_sync(0xffffffffu, clear)) {
           // Both tiles clear the same rows, each before its own second product. (After S_j, so that the
