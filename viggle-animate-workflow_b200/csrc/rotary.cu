@@ -21,6 +21,7 @@ namespace slim {
 namespace rope {
 
 constexpr int THREADS = 256;
+constexpr int BLOCKS = 8;           // blocks per SM: 32 registers a thread
 constexpr int MAX_TOKENS = 16;      // tokens per block
 constexpr int MAX_TABLE = 1024;     // (token, pair) entries of cos/sin in shared memory
 
@@ -68,21 +69,43 @@ struct alignas(sizeof(T) * P) Vec {
   T e[P];
 };
 
+// P pairs: partners in u and v (HALF), or neighbours in u then v.
+template <typename T, int P, bool HALF>
+__device__ __forceinline__ void turn(Vec<T, P>& u, Vec<T, P>& v, const float2* cs, int step) {
+#pragma unroll
+  for (int e = 0; e < P; ++e) {
+    T& xe = HALF || P == 1 ? u.e[e] : 2 * e < P ? u.e[2 * e % P] : v.e[2 * e % P];
+    T& ye = HALF || P == 1 ? v.e[e] : 2 * e < P ? u.e[(2 * e + 1) % P] : v.e[(2 * e + 1) % P];
+    const float2 a = cs[e * step];
+    const float x = to_f<T>(xe), y = to_f<T>(ye);
+    xe = from_f<T>(turn_x(x, y, a));
+    ye = from_f<T>(turn_y(x, y, a));
+  }
+}
+
 // P pairs per item: two accesses of P elements (a half pair's partners, or the two halves of
 // 2P neighbours), P * sizeof(T) bytes each.
 template <typename T, int P, bool HALF>
-__global__ void __launch_bounds__(THREADS) rotary_kernel(const Params p) {
+__global__ void __launch_bounds__(THREADS, BLOCKS) rotary_kernel(const Params p) {
   using V = Vec<T, P>;
   __shared__ float2 table[MAX_TABLE];
+  __shared__ void* rows[MAX_TOKENS][4];  // a token's rows in q, k, q_out, k_out
   const int64_t total = p.batch * p.seq;
   const int64_t first = static_cast<int64_t>(blockIdx.x) * p.tokens;
   const int n_tok = static_cast<int>(total - first < p.tokens ? total - first : p.tokens);
 
+  if (threadIdx.x < n_tok * 4) {
+    const int t = threadIdx.x >> 2, w = threadIdx.x & 3;
+    const slim_view& v = w == 0 ? p.q : w == 1 ? p.k : w == 2 ? p.q_out : p.k_out;
+    const uint32_t token = static_cast<uint32_t>(first) + t, b = token / static_cast<uint32_t>(p.seq);
+    const uint32_t s = token - b * static_cast<uint32_t>(p.seq);
+    rows[t][w] = static_cast<T*>(v.data) + b * v.stride_b + s * v.stride_s;
+  }
   for (int i = threadIdx.x; i < n_tok * p.pairs; i += THREADS) {
     const int t = i / p.pairs;
     const int j = i - t * p.pairs;
-    const int64_t b = (first + t) / p.seq;
-    const int64_t s = first + t - b * p.seq;
+    const uint32_t token = static_cast<uint32_t>(first) + t, b = token / static_cast<uint32_t>(p.seq);
+    const uint32_t s = token - b * static_cast<uint32_t>(p.seq);
     int axis = 0;
     while (axis + 1 < p.axes && j >= p.section_end[axis]) ++axis;
     const int64_t at = b * p.pos_b + s * p.pos_s + axis * p.pos_a;
@@ -97,68 +120,41 @@ __global__ void __launch_bounds__(THREADS) rotary_kernel(const Params p) {
     float sn, cs;
     sincospif(2.0f * static_cast<float>((turns - rint(turns)) + turns_lo), &sn, &cs);
     if (p.inverse) sn = -sn;
-    table[i] = make_float2(cs * p.magnitude, sn * p.magnitude);
+    // the pairs of a work item lie rot_chunks apart: its neighbours' are next to them
+    table[t * p.pairs + j % P * p.rot_chunks + j / P] = make_float2(cs * p.magnitude, sn * p.magnitude);
   }
   __syncthreads();
 
+  // Rows of this block: (token, head); this thread takes chunk c of every rows_step-th. (Two or four rows
+  // in flight a thread cost more in registers, hence threads, than they gain: 293, 381, 625 us at 30026
+  // tokens x 112 heads x 128.)
   const int rows_step = THREADS / p.chunks > 0 ? THREADS / p.chunks : 1;
   for (int c = threadIdx.x % p.chunks; c < p.chunks; c += THREADS) {
     const int row0 = threadIdx.x / p.chunks;
     if (row0 >= rows_step) break;
-    // rows of this block: (token, head); this thread takes chunk c of every rows_step-th
+    const bool turns = c < p.rot_chunks;
+    const int lo = turns ? (HALF ? c * P : 2 * c * P) : p.rot + (c - p.rot_chunks) * P;
+    const int hi = HALF ? c * P + p.pairs : 2 * c * P + P;
     int t = row0 / p.heads;
     int h = row0 - t * p.heads;
     while (t < n_tok) {
-      const int64_t b = (first + t) / p.seq;
-      const int64_t s = first + t - b * p.seq;
       const bool is_k = h >= p.heads_q;
-      const slim_view& in = is_k ? p.k : p.q;
-      const slim_view& out = is_k ? p.k_out : p.q_out;
       const int hh = is_k ? h - p.heads_q : h;
-      const T* src = static_cast<const T*>(in.data) + b * in.stride_b + s * in.stride_s + hh * in.stride_h;
-      T* dst = static_cast<T*>(out.data) + b * out.stride_b + s * out.stride_s + hh * out.stride_h;
-      if (c < p.rot_chunks) {
-        const int j = c * P;
-        const int lo = HALF ? j : 2 * j;
-        const int hi = HALF ? j + p.pairs : 2 * j + P;
-        V u = *reinterpret_cast<const V*>(src + lo);
-        V v = *reinterpret_cast<const V*>(src + hi);
-        const float2* cs = table + t * p.pairs + j;
-        if (HALF) {
-#pragma unroll
-          for (int e = 0; e < P; ++e) {
-            const float2 a = cs[e];
-            const float x = to_f<T>(u.e[e]), y = to_f<T>(v.e[e]);
-            u.e[e] = from_f<T>(turn_x(x, y, a));
-            v.e[e] = from_f<T>(turn_y(x, y, a));
-          }
-        } else if (P == 1) {
-          const float2 a = cs[0];
-          const float x = to_f<T>(u.e[0]), y = to_f<T>(v.e[0]);
-          u.e[0] = from_f<T>(turn_x(x, y, a));
-          v.e[0] = from_f<T>(turn_y(x, y, a));
-        } else {
-#pragma unroll
-          for (int e = 0; e < P; ++e) {
-            T& xe = 2 * e < P ? u.e[(2 * e) % P] : v.e[(2 * e) % P];
-            T& ye = 2 * e < P ? u.e[(2 * e + 1) % P] : v.e[(2 * e + 1) % P];
-            const float2 a = cs[e];
-            const float x = to_f<T>(xe), y = to_f<T>(ye);
-            xe = from_f<T>(turn_x(x, y, a));
-            ye = from_f<T>(turn_y(x, y, a));
-          }
-        }
-        *reinterpret_cast<V*>(dst + lo) = u;
-        *reinterpret_cast<V*>(dst + hi) = v;
-      } else {
-        const int e0 = p.rot + (c - p.rot_chunks) * P;
-        *reinterpret_cast<V*>(dst + e0) = *reinterpret_cast<const V*>(src + e0);
-      }
+      const T* src = static_cast<const T*>(rows[t][is_k]) + hh * (is_k ? p.k.stride_h : p.q.stride_h);
+      T* dst = static_cast<T*>(rows[t][2 + is_k]) + hh * (is_k ? p.k_out.stride_h : p.q_out.stride_h);
+      const float2* cs = table + t * p.pairs + c;
+      V u = *reinterpret_cast<const V*>(src + lo), v;
+      if (turns) v = *reinterpret_cast<const V*>(src + hi);
       h += rows_step;
       while (h >= p.heads) {
         h -= p.heads;
         ++t;
       }
+      if (turns) {
+        turn<T, P, HALF>(u, v, cs, p.rot_chunks);
+        *reinterpret_cast<V*>(dst + hi) = v;
+      }
+      *reinterpret_cast<V*>(dst + lo) = u;
     }
   }
 }
@@ -197,13 +193,18 @@ cudaError_t launch(Params& p, bool half, bool copies, cudaStream_t st) {
   }
   p.rot_chunks = p.pairs / P;
   p.chunks = p.rot_chunks + (copies ? (p.dim - p.rot) / P : 0);
-  // Tokens per block: about four rounds of its threads, within the table.
+  // Tokens per block: up to twelve rounds of its threads, so that the table's latency is a small part (four
+  // took 307 us at 30026 tokens x 112 heads x 128, twelve 293 us), within the table; fewer where that leaves
+  // SMs idle, or a second round of blocks with few in it (8198 tokens x 48 heads: 47 us with two tokens a
+  // block, 51 with five).
   const int64_t items = static_cast<int64_t>(p.heads) * p.chunks;
-  int64_t tokens = (4 * THREADS + items - 1) / items;
+  int64_t tokens = (12 * THREADS + items - 1) / items;
   if (tokens > MAX_TOKENS) tokens = MAX_TOKENS;
   if (tokens > MAX_TABLE / p.pairs) tokens = MAX_TABLE / p.pairs;
   const int64_t total = p.batch * p.seq;
-  while (tokens > 1 && total / tokens < 148 * 4) tokens >>= 1;  // few tokens: spread them over the SMs first
+  const int64_t sms = sm_count(), full = sms * BLOCKS;
+  auto uneven = [&](int64_t blocks) { return blocks < sms * 4 || (blocks > full && blocks < 2 * full); };
+  while (tokens > 1 && uneven(total / tokens)) tokens >>= 1;
   p.tokens = static_cast<int>(tokens < 1 ? 1 : tokens);
   if constexpr (sizeof(T) == 2)
     if (P == 8) return launch_p<T, 8>(p, half, st);
