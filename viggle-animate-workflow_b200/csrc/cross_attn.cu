@@ -90,7 +90,8 @@ cudaError_t launch(const Params& p, const Plan& plan, float* partial, cudaStream
     return cudaErrorInvalidValue;
   const int64_t per_head = plan.splits > 0 ? plan.q_tiles * plan.splits : (plan.q_tiles + 1) / 2;
   const int64_t items = per_head * p.kv_heads * p.batch;
-  const TileParams tp{p.out, p.q_len, p.kv_len, p.kv_heads, p.dim, plan.group, plan.tokens, p.k.stride_b != 0,
+  const TileParams tp{p.out, p.q_len, p.kv_len, p.kv_heads, p.dim, plan.group, plan.tokens,
+                      static_cast<uint32_t>((65536 + plan.group - 1) / plan.group), p.k.stride_b != 0,
                       p.k.stride_h != 0, p.v.stride_b != 0, p.v.stride_h != 0, p.scale2, p.keys,
                       static_cast<int>(items), static_cast<int>(per_head), plan.splits, plan.per, plan.rows, partial};
   const int64_t sms = sm_count();

@@ -134,6 +134,7 @@ struct TileParams {
   int64_t q_len, kv_len;
   int kv_heads, dim;
   int group, tokens;          // query heads per key head, tokens per row tile
+  uint32_t group_inv;         // ceil(2^16 / group): row / group = row * group_inv >> 16 for rows below 128
   int kb, kh, vb, vh;         // 0 for a k / v that is the same for every sequence / head
   float scale2;
   Keys keys;
@@ -142,6 +143,8 @@ struct TileParams {
   int rows;                   // split: rows of a tile that exist
   float* partial;             // split: results of the pieces
 };
+
+__device__ __forceinline__ int token_of(const TileParams& p, int row) { return row * p.group_inv >> 16; }
 
 template <bool BIAS>
 __device__ __forceinline__ int keys_of(const TileParams& p, int b) {

@@ -349,6 +349,8 @@ narrow_kernel(const __grid_constant__ CUtensorMap tq, const __grid_constant__ CU
       // at u ^ (r >> 2 & 1)), then 32-byte pieces of 16 rows a store
       const float inv = l == 0.0f ? 0.0f : 1.0f / l;
       uint8_t* stage = smem + L::OFF_STAGING + warp * L::STAGING;
+      const int tokens = p.q_len - it.tok0 < p.tokens ? static_cast<int>(p.q_len - it.tok0) : p.tokens;
+      T* out = static_cast<T*>(p.out.data) + it.b * p.out.stride_b + it.tok0 * p.out.stride_s + it.hk * p.group * p.out.stride_h;
 #pragma unroll
       for (int c = 0; c < L::OUT_COLS; c += 16) {
         __syncwarp();
@@ -366,11 +368,9 @@ narrow_kernel(const __grid_constant__ CUtensorMap tq, const __grid_constant__ CU
 #pragma unroll
           for (int i = 0; i < 2; ++i) {
             const int sr = i * 16 + (lane >> 1), tr = quarter * 32 + sr;
-            const int tok = tr / p.group, head = it.hk * p.group + tr - tok * p.group;
-            const int64_t token = it.tok0 + tok;
-            if (tok < p.tokens && token < p.q_len)
-              *reinterpret_cast<uint4*>(static_cast<T*>(p.out.data) + it.b * p.out.stride_b + token * p.out.stride_s +
-                                        head * p.out.stride_h + col) =
+            const int tok = token_of(p, tr);
+            if (tok < tokens)
+              *reinterpret_cast<uint4*>(out + tok * p.out.stride_s + (tr - tok * p.group) * p.out.stride_h + col) =
                   *reinterpret_cast<const uint4*>(stage + sr * 32 + ((chunk ^ (sr >> 2 & 1)) << 4));
           }
         }

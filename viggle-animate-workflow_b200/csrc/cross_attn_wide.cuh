@@ -299,10 +299,13 @@ wide_kernel(const __grid_constant__ CUtensorMap tq, const __grid_constant__ CUte
     uint32_t steps = 0;  // of this tile before the item
     uint32_t h = 0;      // of both tiles before the item
     uint32_t items = 0;  // of this tile before the item
+    Item next{};
+    if (blockIdx.x < p.items) next = item_at<BIAS>(p, blockIdx.x);
 #pragma unroll 1
     for (int index = blockIdx.x; index < p.items; index += gridDim.x) {
-      const Item it = item_at<BIAS>(p, index);
+      const Item it = next;
       if (t >= it.tiles) {
+        if (index + gridDim.x < p.items) next = item_at<BIAS>(p, index + gridDim.x);
         h += it.steps;
         continue;
       }
@@ -360,12 +363,16 @@ wide_kernel(const __grid_constant__ CUtensorMap tq, const __grid_constant__ CUte
         __syncwarp();
         if (lane == 0) mbar_arrive(&sh.p_full[t]);
       }
+      if (index + gridDim.x < p.items) next = item_at<BIAS>(p, index + gridDim.x);  // ahead of its use: it loads
       const float own_l = l2.x + l2.y, l = own_l + other(own_l);
       if (it.steps > 0) wait(&sh.o_full[t], items++ & 1);
       // 32 columns of the warp's 32 rows at a time through its own shared memory (16-byte chunk u of row
       // r at u ^ (r >> 1 & 3)), then 64-byte pieces of 8 rows a store
       const float inv = l == 0.0f ? 0.0f : 1.0f / l;
       uint8_t* stage = smem + L::OFF_STAGING + warp * L::STAGING;
+      const int64_t token0 = it.tok0 + t * p.tokens;
+      const int tokens = p.q_len - token0 < p.tokens ? static_cast<int>(p.q_len - token0) : p.tokens;
+      T* out = static_cast<T*>(p.out.data) + it.b * p.out.stride_b + token0 * p.out.stride_s + it.hk * p.group * p.out.stride_h;
 #pragma unroll 1
       for (int c = 0; c < DP / 2; c += 32) {
         uint32_t r[32];
@@ -397,11 +404,9 @@ wide_kernel(const __grid_constant__ CUtensorMap tq, const __grid_constant__ CUte
 #pragma unroll
           for (int i = 0; i < 4; ++i) {
             const int sr = i * 8 + (lane >> 2), tr = quarter * 32 + sr;
-            const int tok = tr / p.group, head = it.hk * p.group + tr - tok * p.group;
-            const int64_t token = it.tok0 + t * p.tokens + tok;
-            if (tok < p.tokens && token < p.q_len)
-              *reinterpret_cast<uint4*>(static_cast<T*>(p.out.data) + it.b * p.out.stride_b + token * p.out.stride_s +
-                                        head * p.out.stride_h + col) =
+            const int tok = token_of(p, tr);
+            if (tok < tokens)
+              *reinterpret_cast<uint4*>(out + tok * p.out.stride_s + (tr - tok * p.group) * p.out.stride_h + col) =
                   *reinterpret_cast<const uint4*>(stage + sr * 64 + ((chunk ^ (sr >> 1 & 3)) << 4));
           }
         }

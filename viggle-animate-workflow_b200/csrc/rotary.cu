@@ -117,9 +117,12 @@ __global__ void __launch_bounds__(THREADS, BLOCKS) rotary_kernel(const Params p)
     const double f = p.inv_freq[j];
     const double g = f * kTurn, g_lo = fma(f, kTurn, -g) + f * kTurnLo;
     const double turns = pos * g, turns_lo = fma(pos, g, -turns) + pos * g_lo;
-    float sn, cs;
-    sincospif(2.0f * static_cast<float>((turns - rint(turns)) + turns_lo), &sn, &cs);
-    if (p.inverse) sn = -sn;
+    // sin and cos of the fraction rounded to fp32, then moved by what the rounding left
+    const double part = (turns - rint(turns)) + turns_lo;
+    const float near = static_cast<float>(part), left = 6.2831853f * static_cast<float>(part - near);
+    float s0, c0;
+    sincospif(2.0f * near, &s0, &c0);
+    const float cs = fmaf(-left, s0, c0), sn = p.inverse ? -fmaf(left, c0, s0) : fmaf(left, c0, s0);
     // the pairs of a work item lie rot_chunks apart: its neighbours' are next to them
     table[t * p.pairs + j % P * p.rot_chunks + j / P] = make_float2(cs * p.magnitude, sn * p.magnitude);
   }
