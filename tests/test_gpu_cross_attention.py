@@ -174,6 +174,53 @@ def test_lowest_values_mask_and_a_row_of_them_is_no_mask(cuda, kind, sq):
     check(out, q, k, v, bias)
 
 
+@pytest.mark.parametrize("d", [64, 128])
+@pytest.mark.parametrize("sq", [100, 300])   # one row tile, and pairs of them with a single one at the end
+@pytest.mark.parametrize("kind", ["none", "lengths", "bool", "additive"])
+def test_many_items_of_all_lengths_on_one_sm(cuda, kind, sq, d):
+    """More (sequence, head, rows) pieces than SMs, so that a CTA goes from one to the next: sequences
+    without keys, of one key, of whole tiles and of several."""
+    lens = [0, 640, 1, 128, 513, 0, 300, 77]
+    b, h, sk = len(lens), 40, 640
+    q, k, v = inputs(cuda, "bf16", b, sq, sk, h, h, d)
+    lengths = torch.tensor(lens, device=cuda)
+    keep = torch.arange(sk, device=cuda) < lengths[:, None]
+    bias = torch.where(keep, 0.0, -math.inf)
+    args = {}
+    if kind == "none":
+        bias = None
+    elif kind == "lengths":
+        args["kv_lengths"] = lengths
+    elif kind == "bool":
+        args["key_mask"] = keep
+    else:
+        bias = torch.where(keep, torch.randn(b, sk, device=cuda), -math.inf)
+        args["key_mask"] = bias
+    if bias is not None:
+        k[~keep], v[~keep] = math.nan, math.nan
+    out = attention.cross_attention(q, k, v, **args)
+    check(out, q, k, v, bias)
+    for _ in range(3):
+        assert torch.equal(attention.cross_attention(q, k, v, **args), out)
+
+
+@pytest.mark.parametrize("sq", [1, 300])
+def test_offsets_past_32_bits(cuda, sq):
+    """Rows more than 2^31 elements apart (a long cache of which a part is read)."""
+    buf = torch.empty((1 << 31) + (1 << 22), device=cuda, dtype=torch.bfloat16)
+    far = torch.as_strided(buf, (2, 500, 2, 64), (1 << 31, 128, 64, 1))
+    q, k, v = inputs(cuda, "bf16", 2, sq, 500, 2, 2, 64)
+    far.copy_(k)
+    want = attention.cross_attention(q, k, v)
+    assert torch.equal(attention.cross_attention(q, far, v), want)
+    far.copy_(v)
+    assert torch.equal(attention.cross_attention(q, k, far), want)
+    out = ops.rotary(far, None, torch.arange(500, device=cuda), torch.ones(32, device=cuda))
+    assert torch.equal(out, ops.rotary(v, None, torch.arange(500, device=cuda), torch.ones(32, device=cuda)))
+    ops.rotary(far, None, torch.arange(500, device=cuda), torch.ones(32, device=cuda), inplace=True)
+    assert torch.equal(far, out)
+
+
 def test_masks_and_lengths_together_and_shared_masks(cuda):
     q, k, v = inputs(cuda, "bf16", 3, 20, 260, 4, 2, 64)
     mask = torch.rand(260, device=cuda) < 0.5

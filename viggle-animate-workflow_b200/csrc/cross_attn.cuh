@@ -26,7 +26,6 @@ constexpr float kLog2e = 1.4426950408889634f;
 constexpr int MAX_DIM = 128;
 constexpr int KEY_TILE = 128;
 
-
 // Which keys take part. A boolean mask and lengths are read by the attention kernel itself; an additive
 // mask goes through bias_kernel first (then lengths are in n_keys, and mask and lengths are null).
 struct Keys {
