@@ -9,7 +9,9 @@
 // tokens: it computes their cos and sin once into shared memory (the angle reduced to turns in
 // fp64, because pos * inv_freq in fp32 is off by up to 2^-24 of the whole angle, not of a turn),
 // then all heads of q and k go through in 16-byte accesses. The products and sums are fp32,
-// rounded once to the element type.
+// rounded once to the element type. 30026 tokens x 112 heads x 128, 96 of them turned, bf16 rows of
+// a packed buffer: 272 us, 6.3 TB/s; by single elements instead of words it took 293 us, as the
+// kernel is then close to being bound by instruction issue (70 % of the slots).
 #include <cuda_bf16.h>
 #include <cuda_fp16.h>
 #include <cuda_runtime.h>
@@ -69,9 +71,52 @@ struct alignas(sizeof(T) * P) Vec {
   T e[P];
 };
 
-// P pairs: partners in u and v (HALF), or neighbours in u then v.
+// Two 16-bit elements of a word as fp32, and back.
+template <typename T>
+__device__ __forceinline__ float2 unpack2(uint32_t w);
+template <>
+__device__ __forceinline__ float2 unpack2<__nv_bfloat16>(uint32_t w) {
+  return make_float2(__uint_as_float(w << 16), __uint_as_float(w & 0xffff0000u));
+}
+template <>
+__device__ __forceinline__ float2 unpack2<__half>(uint32_t w) { return __half22float2(*reinterpret_cast<const __half2*>(&w)); }
+template <typename T>
+__device__ __forceinline__ uint32_t pack2(float lo, float hi);
+template <>
+__device__ __forceinline__ uint32_t pack2<__nv_bfloat16>(float lo, float hi) {
+  const __nv_bfloat162 h = __floats2bfloat162_rn(lo, hi);
+  return *reinterpret_cast<const uint32_t*>(&h);
+}
+template <>
+__device__ __forceinline__ uint32_t pack2<__half>(float lo, float hi) {
+  const __half2 h = __floats2half2_rn(lo, hi);
+  return *reinterpret_cast<const uint32_t*>(&h);
+}
+
+// P pairs: partners in u and v (HALF), or neighbours in u then v. cs[e * step]: (cos, sin) of pair e.
 template <typename T, int P, bool HALF>
 __device__ __forceinline__ void turn(Vec<T, P>& u, Vec<T, P>& v, const float2* cs, int step) {
+  if constexpr (sizeof(T) == 2 && P >= 2) {  // by words: the kernel is close to being bound by issue
+    uint32_t* uw = reinterpret_cast<uint32_t*>(&u);
+    uint32_t* vw = reinterpret_cast<uint32_t*>(&v);
+    if constexpr (HALF) {
+#pragma unroll
+      for (int w = 0; w < P / 2; ++w) {
+        const float2 x = unpack2<T>(uw[w]), y = unpack2<T>(vw[w]);
+        const float2 a = cs[2 * w * step], b = cs[(2 * w + 1) * step];
+        uw[w] = pack2<T>(turn_x(x.x, y.x, a), turn_x(x.y, y.y, b));
+        vw[w] = pack2<T>(turn_y(x.x, y.x, a), turn_y(x.y, y.y, b));
+      }
+    } else {
+#pragma unroll
+      for (int e = 0; e < P; ++e) {
+        uint32_t& word = e < P / 2 ? uw[e % (P / 2)] : vw[e % (P / 2)];
+        const float2 z = unpack2<T>(word), a = cs[e * step];
+        word = pack2<T>(turn_x(z.x, z.y, a), turn_y(z.x, z.y, a));
+      }
+    }
+    return;
+  }
 #pragma unroll
   for (int e = 0; e < P; ++e) {
     T& xe = HALF || P == 1 ? u.e[e] : 2 * e < P ? u.e[2 * e % P] : v.e[2 * e % P];
@@ -197,7 +242,7 @@ cudaError_t launch(Params& p, bool half, bool copies, cudaStream_t st) {
   p.rot_chunks = p.pairs / P;
   p.chunks = p.rot_chunks + (copies ? (p.dim - p.rot) / P : 0);
   // Tokens per block: up to twelve rounds of its threads, so that the table's latency is a small part (four
-  // took 307 us at 30026 tokens x 112 heads x 128, twelve 293 us), within the table; fewer where that leaves
+  // took 14 us more at 30026 tokens x 112 heads x 128), within the table; fewer where that leaves
   // SMs idle, or a second round of blocks with few in it (8198 tokens x 48 heads: 47 us with two tokens a
   // block, 51 with five).
   const int64_t items = static_cast<int64_t>(p.heads) * p.chunks;

@@ -15,6 +15,8 @@ The packed [S, 3*H*D] bf16 buffer the DiT splits into q/k/v views is read in pla
 than ``min_seq``) go back to the model's own attention, as in the reference
 (attention_triton.py:253-263, 301-305). There is no CPU path: ``attention_packed`` raises
 ``NativeUnavailable`` without the library and an sm_100 GPU.
+
+``cross_attention`` attends to the keys and values of another sequence, unquantised (bf16/fp16).
 """
 
 from __future__ import annotations
