@@ -29,7 +29,7 @@ def call(dtype=_native.BF16, b=2, sq=4, sk=8, h=2, hk=2, d=64, q=None, k=None, o
     (dict(h=0), _native.SLIM_ERR_SHAPE), (dict(sk=-1), _native.SLIM_ERR_SHAPE),
     (dict(sq=1 << 31), _native.SLIM_ERR_SHAPE), (dict(b=1 << 16), _native.SLIM_ERR_SHAPE),
     (dict(scale=0.0), _native.SLIM_ERR_SHAPE), (dict(scale=float("nan")), _native.SLIM_ERR_SHAPE),
-    (dict(scale=float("inf")), _native.SLIM_ERR_SHAPE),
+    (dict(scale=float("inf")), _native.SLIM_ERR_SHAPE), (dict(scale=3e38), _native.SLIM_ERR_SHAPE),
     (dict(q=view(0)), _native.SLIM_ERR_NULL), (dict(k=view(0)), _native.SLIM_ERR_NULL),
     (dict(q=view(18)), _native.SLIM_ERR_ALIGN), (dict(k=view(s=65)), _native.SLIM_ERR_ALIGN),
     (dict(out=view(h=4)), _native.SLIM_ERR_ALIGN),

@@ -357,6 +357,8 @@ def test_refusals(cuda):
         (lambda: attention.cross_attention(q, k, v, key_mask=torch.ones(2, 1, 5, 8, device=cuda, dtype=torch.bool)), ValueError),
         (lambda: attention.cross_attention(q, k, v, key_mask=torch.ones(2, 8, device=cuda, dtype=torch.int64)), TypeError),
         (lambda: attention.cross_attention(q, k, v, key_mask=torch.ones(2, 8, dtype=torch.bool)), ValueError),
+        (lambda: attention.cross_attention(q, k, v, key_mask=[True] * 8), TypeError),
+        (lambda: attention.cross_attention(q, k, v, kv_lengths=[8, 8]), TypeError),
         (lambda: attention.cross_attention(q, k, v, kv_lengths=lengths.float()), TypeError),
         (lambda: attention.cross_attention(q, k, v, kv_lengths=lengths[:1]), ValueError),
         (lambda: attention.cross_attention(q, k, v, kv_lengths=lengths.cpu()), ValueError),

@@ -193,7 +193,7 @@ int slim_cross_attn(const slim_view* q, const slim_view* k, const slim_view* v, 
     return fail(SLIM_ERR_DTYPE, "unsupported mask type %d", mask_type);
   if (kv_lengths != nullptr && lengths_bits != 32 && lengths_bits != 64)
     return fail(SLIM_ERR_DTYPE, "lengths must be 32- or 64-bit integers");
-  if (!(scale > 0.0f) || !(scale <= FLT_MAX)) return fail(SLIM_ERR_SHAPE, "scale must be positive and finite");
+  if (!(scale > 0.0f) || !(scale * xattn::kLog2e <= FLT_MAX)) return fail(SLIM_ERR_SHAPE, "scale must be positive and finite");
   if (batch == 0 || q_len == 0) return SLIM_OK;
   if (q == nullptr || k == nullptr || v == nullptr || out == nullptr || q->data == nullptr || out->data == nullptr ||
       (kv_len > 0 && (k->data == nullptr || v->data == nullptr)))

@@ -529,7 +529,7 @@ def _no_grad(*tensors) -> None:
     if not torch.is_grad_enabled():
         return
     for t in tensors:
-        if t is not None and t.requires_grad:
+        if getattr(t, "requires_grad", False):
             raise ValueError("this operator has no backward pass; call it under torch.no_grad() or detach its inputs")
 
 
