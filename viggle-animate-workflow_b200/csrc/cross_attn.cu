@@ -39,7 +39,7 @@ struct Plan {
 // The cheapest layout by a count of steps, one row tile x one key tile in the narrow kernel (about 1.25 us).
 // The wide kernel takes two row tiles x one key tile in 1.6 of them and moves half the keys and values: it
 // wins as soon as there are enough pairs of row tiles for the SMs. An item's ends cost 1. Pieces cost a
-// second launch and their sums through memory: 4, and one more for every 4 MB.
+// second launch and their sums through memory: 6, and one more for every 4 MB.
 inline Plan make_plan(int64_t batch, int64_t q_len, int64_t kv_len, int heads, int kv_heads, int dim) {
   Plan p{};
   p.group = heads / kv_heads;
@@ -54,7 +54,7 @@ inline Plan make_plan(int64_t batch, int64_t q_len, int64_t kv_len, int heads, i
     const int64_t per = (nk + s - 1) / s;
     if (s > 1 && (s - 1) * per >= nk) continue;  // the last pieces would be empty
     double cost = static_cast<double>((tiles * s + sms - 1) / sms * (per + 1));
-    if (s > 1) cost += 4.0 + static_cast<double>(narrow::split_floats(s, tiles, p.rows, dp)) / (1 << 20);
+    if (s > 1) cost += 6.0 + static_cast<double>(narrow::split_floats(s, tiles, p.rows, dp)) / (1 << 20);
     if (cost < best) {
       best = cost;
       p.splits = static_cast<int>(s);
