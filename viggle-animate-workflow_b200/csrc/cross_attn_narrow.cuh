@@ -427,6 +427,7 @@ narrow_kernel(const __grid_constant__ CUtensorMap tq, const __grid_constant__ CU
             if (fresh) break;
             fresh = named_barrier_any(1 + quarter, 128, real && max_of<32>(y) * sc > m + GROWTH);
             if (!fresh) break;
+            tmem_st_wait();  // stores are not ordered: these weights have landed before the next go over them
           }
           l2 = add2(l2, add);
           tmem_st_wait();
