@@ -56,3 +56,14 @@ PIECES = [(1, 130, 2560, 20, 20, 128), (2, 40, 2500, 30, 10, 64)]
 @pytest.mark.parametrize("shape", NARROW + PIECES)
 def test_a_maximum_that_grows_within_a_row_tile(cuda, shape, kind, dtype):
     run(cuda, dtype, kind, *shape)
+
+
+# pairs of row tiles, and (9 of them) a single one at the end
+WIDE = [(2, 1000, 1000, 40, 40, 64), (2, 1100, 640, 40, 40, 128), (1, 1300, 700, 48, 24, 72)]
+
+
+@pytest.mark.parametrize("dtype", ["bf16", "f16"])
+@pytest.mark.parametrize("kind", ["none", "bool", "additive"])
+@pytest.mark.parametrize("shape", WIDE)
+def test_a_maximum_that_grows_within_a_pair_of_row_tiles(cuda, shape, kind, dtype):
+    run(cuda, dtype, kind, *shape)

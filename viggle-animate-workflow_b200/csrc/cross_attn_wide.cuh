@@ -334,6 +334,7 @@ wide_kernel(const __grid_constant__ CUtensorMap tq, const __grid_constant__ CUte
         mask_scores<BIAS, 64>(p, it.b, key0, 64 * half, bits, y);
         const float own = max_of<64>(y) * sc;
         // (the barrier also tells that both halves have read the scores that the weights go over)
+        tc_fence_before();
         if (j == 0 || named_barrier_any(pair, 64, real && own > m + GROWTH)) {
           const float m_new = fmaxf(m, fmaxf(own, other(own)));
           if (j > 0) {  // O holds P_0 V_0 + ... + P_{j-1} V_{j-1} (done before S_j)
@@ -343,6 +344,7 @@ wide_kernel(const __grid_constant__ CUtensorMap tq, const __grid_constant__ CUte
           }
           m = m_new;
         }
+        tc_fence_after();
         const float off = m == -INFINITY ? 0.0f : -m;
 #pragma unroll
         for (int c = 0; c < 64; c += 32) {
