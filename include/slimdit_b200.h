@@ -338,6 +338,12 @@ int slim_rotary(const slim_view* q, const slim_view* q_out, int heads_q, const s
 int slim_cross_attn_workspace_bytes(int64_t batch, int64_t q_len, int64_t kv_len, int heads,
                                     int kv_heads, int dim, int additive, uint64_t* bytes);
 
+/* How slim_cross_attn lays such a call over the current device: pieces 0 = two row tiles a CTA with all
+ * their keys, 1 = one row tile a CTA, n > 1 = the keys of a row tile in n pieces on several SMs;
+ * key_tiles = the most tiles of 128 keys that a CTA goes through for one of them. */
+int slim_cross_attn_layout(int64_t batch, int64_t q_len, int64_t kv_len, int heads, int kv_heads,
+                           int dim, int* pieces, int* key_tiles);
+
 /* mask (or NULL): per key, element (b, i) at b * mask_stride_b + i * mask_stride_k; SLIM_MASK_BOOL
  * or an additive SLIM_F32/BF16/F16 whose -inf excludes the key. kv_lengths (or NULL): device
  * [batch] of 32- or 64-bit integers; keys from there on are excluded (clamped to 0..kv_len). What

@@ -47,3 +47,18 @@ def test_workspace_sizes():
     assert n.value >= 2 * 128 * 4 + 2 * 4
     assert lib.slim_cross_attn_workspace_bytes(2, 300, 77, 4, 4, 64, 1, None) == _native.SLIM_ERR_NULL
     assert lib.slim_cross_attn_workspace_bytes(2, 300, 77, 4, 3, 64, 1, ctypes.byref(n)) == _native.SLIM_ERR_SHAPE
+
+
+def layout(*shape):
+    pieces, tiles = ctypes.c_int(-1), ctypes.c_int(-1)
+    rc = _native.load().slim_cross_attn_layout(*shape, ctypes.byref(pieces), ctypes.byref(tiles))
+    return rc, pieces.value, tiles.value
+
+
+def test_layouts():
+    assert layout(1, 4096, 4096, 40, 40, 128) == (_native.SLIM_OK, 0, 32)   # enough pairs of row tiles
+    assert layout(1, 1, 200, 8, 8, 64) == (_native.SLIM_OK, 1, 2)           # too few keys to cut
+    rc, pieces, tiles = layout(1, 1, 131071, 32, 8, 128)
+    assert rc == _native.SLIM_OK and 1 < pieces <= 128 and (pieces - 1) * tiles < 1024 <= pieces * tiles
+    assert layout(2, 300, 77, 4, 3, 64)[0] == _native.SLIM_ERR_SHAPE
+    assert _native.load().slim_cross_attn_layout(1, 1, 1, 1, 1, 64, None, None) == _native.SLIM_ERR_NULL

@@ -5,12 +5,13 @@ The tolerance is the one of test_gpu_cross_attention.py, per output element. The
 weights grow, so that a tile's share of the result stays within what the tolerance tells apart.
 """
 
+import ctypes
 import math
 
 import pytest
 import torch
 
-from slimdit import attention
+from slimdit import _native, attention
 from test_gpu_cross_attention import check, inputs
 
 pytestmark = pytest.mark.gpu
@@ -27,6 +28,13 @@ def rising(cuda, dtype, b, sq, sk, h, hk, d):
     k[..., 0] = (6 * tile)[:, None].to(k.dtype)
     v = (v.float() * torch.exp2(tile * (-8 if dtype == "bf16" else -2))[:, None, None]).to(v.dtype)
     return q, k, v
+
+
+def layout(b, sq, sk, h, hk, d):
+    """(pieces of a row tile's keys, 0 for pairs of row tiles; most key tiles of one)"""
+    pieces, tiles = ctypes.c_int(), ctypes.c_int()
+    _native.check(_native.load().slim_cross_attn_layout(b, sq, sk, h, hk, d, pieces, tiles))
+    return pieces.value, tiles.value
 
 
 def run(cuda, dtype, kind, b, sq, sk, h, hk, d):
@@ -55,6 +63,8 @@ PIECES = [(1, 130, 2560, 20, 20, 128), (2, 40, 2500, 30, 10, 64)]
 @pytest.mark.parametrize("kind", ["none", "bool", "additive"])
 @pytest.mark.parametrize("shape", NARROW + PIECES)
 def test_a_maximum_that_grows_within_a_row_tile(cuda, shape, kind, dtype):
+    pieces, tiles = layout(*shape)
+    assert tiles >= 3 and (pieces == 1 if shape in NARROW else pieces > 1), "the shape no longer gives this layout"
     run(cuda, dtype, kind, *shape)
 
 
@@ -66,4 +76,5 @@ WIDE = [(2, 1000, 1000, 40, 40, 64), (2, 1100, 640, 40, 40, 128), (1, 1300, 700,
 @pytest.mark.parametrize("kind", ["none", "bool", "additive"])
 @pytest.mark.parametrize("shape", WIDE)
 def test_a_maximum_that_grows_within_a_pair_of_row_tiles(cuda, shape, kind, dtype):
+    assert layout(*shape)[0] == 0 and layout(*shape)[1] >= 5, "the shape no longer gives this layout"
     run(cuda, dtype, kind, *shape)

@@ -181,6 +181,17 @@ int slim_cross_attn_workspace_bytes(int64_t batch, int64_t q_len, int64_t kv_len
   return SLIM_OK;
 }
 
+int slim_cross_attn_layout(int64_t batch, int64_t q_len, int64_t kv_len, int heads, int kv_heads, int dim, int* pieces,
+                           int* key_tiles) {
+  const int rc = xattn::checks(batch, q_len, kv_len, heads, kv_heads, dim);
+  if (rc != SLIM_OK) return rc;
+  if (pieces == nullptr || key_tiles == nullptr) return fail(SLIM_ERR_NULL, "pieces/key_tiles is NULL");
+  const xattn::Plan plan = xattn::make_plan(batch, q_len, kv_len, heads, kv_heads, dim);
+  *pieces = plan.splits;
+  *key_tiles = plan.splits > 0 ? plan.per : static_cast<int>((kv_len + xattn::KEY_TILE - 1) / xattn::KEY_TILE);
+  return SLIM_OK;
+}
+
 int slim_cross_attn(const slim_view* q, const slim_view* k, const slim_view* v, const slim_view* out, int dtype,
                     int64_t batch, int64_t q_len, int64_t kv_len, int heads, int kv_heads, int dim, const void* mask,
                     int mask_type, int64_t mask_stride_b, int64_t mask_stride_k, const void* kv_lengths,
