@@ -62,3 +62,6 @@ def test_layouts():
     assert rc == _native.SLIM_OK and 1 < pieces <= 128 and (pieces - 1) * tiles < 1024 <= pieces * tiles
     assert layout(2, 300, 77, 4, 3, 64)[0] == _native.SLIM_ERR_SHAPE
     assert _native.load().slim_cross_attn_layout(1, 1, 1, 1, 1, 64, None, None) == _native.SLIM_ERR_NULL
+    # one row tile a key head: never paired, however many there are
+    assert layout(74, 1, 2048, 32, 8, 128)[1:] == layout(75, 1, 2048, 32, 8, 128)[1:] == (1, 16)
+    assert layout(4000, 100, 300, 8, 8, 64)[1:] == (1, 3)

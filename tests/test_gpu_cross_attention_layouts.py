@@ -55,7 +55,8 @@ def run(cuda, dtype, kind, b, sq, sk, h, hk, d):
     check(attention.cross_attention(q, k, v, key_mask=mask), q, k, v, bias)
 
 
-NARROW = [(1, 130, 640, 2, 2, 64), (1, 130, 640, 2, 2, 128), (2, 50, 600, 6, 2, 128), (1, 1, 700, 8, 8, 64)]
+NARROW = [(1, 130, 640, 2, 2, 64), (1, 130, 640, 2, 2, 128), (2, 50, 600, 6, 2, 128), (1, 1, 700, 8, 8, 64),
+          (301, 1, 600, 2, 2, 64), (75, 3, 390, 16, 8, 128)]   # more row tiles than four an SM, one a key head
 PIECES = [(1, 130, 2560, 20, 20, 128), (2, 40, 2500, 30, 10, 64)]
 
 

@@ -50,7 +50,13 @@ inline Plan make_plan(int64_t batch, int64_t q_len, int64_t kv_len, int heads, i
   const int64_t pairs = base * ((p.q_tiles + 1) / 2);
   const int dp = dim > 64 ? 128 : 64;
   double best = static_cast<double>((pairs + sms - 1) / sms) * (1.0 + 1.6 * static_cast<double>(nk));
-  for (int64_t s = 1; s <= 128 && s <= (nk > 0 ? nk : 1) && tiles * s <= 4 * sms; ++s) {
+  // The narrow kernel is considered up to 4 row tiles an SM, and for any number of them where a key head has a
+  // single one, as the wide kernel's second tile would then be empty: one query over 2048 keys, 75 sequences of
+  // 32 / 8 heads of 128, 131 us (wide 154); 100 queries over 300, 100 sequences of 8 heads, 47 us (55). With three row
+  // tiles a key head it is no rule: 300 queries over 1000 keys x 296 heads 84 us (90), over 4000 x 2 x 148 heads of
+  // 64 256 us (227).
+  const int64_t most = p.q_tiles == 1 && tiles > 4 * sms ? tiles : 4 * sms;
+  for (int64_t s = 1; s <= 128 && s <= (nk > 0 ? nk : 1) && tiles * s <= most; ++s) {
     const int64_t per = (nk + s - 1) / s;
     if (s > 1 && (s - 1) * per >= nk) continue;  // the last pieces would be empty
     double cost = static_cast<double>((tiles * s + sms - 1) / sms * (per + 1));
