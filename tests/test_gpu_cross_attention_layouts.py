@@ -79,3 +79,33 @@ WIDE = [(2, 1000, 1000, 40, 40, 64), (2, 1100, 640, 40, 40, 128), (1, 1300, 700,
 def test_a_maximum_that_grows_within_a_pair_of_row_tiles(cuda, shape, kind, dtype):
     assert layout(*shape)[0] == 0 and layout(*shape)[1] >= 5, "the shape no longer gives this layout"
     run(cuda, dtype, kind, *shape)
+
+
+@pytest.mark.parametrize("shape", [NARROW[0], PIECES[0], WIDE[1]])
+@pytest.mark.parametrize("at", [0, 77, -1])
+@pytest.mark.parametrize("kind", ["none", "additive"])
+def test_a_long_tail_behind_one_key_that_takes_nearly_all(cuda, shape, at, kind):
+    """One key about 2^25 times as heavy as each of the others, its value 0: what is left is the tail's. Logits
+    without rounding (one element of q and k, scale 1). The largest weight of a row is held as 2^7 or more, so a
+    tiny weight is off by half a step of fp16, 2^-25, over 2^7 of the largest; the other roundings as in
+    test_gpu_cross_attention.py."""
+    b, sq, sk, h, hk, d = shape
+    _, _, v = inputs(cuda, "f16", *shape)
+    q, k = torch.zeros(b, sq, h, d, device=cuda).half(), torch.zeros(b, sk, hk, d, device=cuda).half()
+    q[..., 0] = (1 - 0.03 * (torch.arange(sq, device=cuda) % 4))[:, None].half()
+    k[:, at, :, 0] = 17.5
+    v[:, at] = 0
+    bias = torch.linspace(-1, 0, sk, device=cuda)[None].expand(b, sk) if kind == "additive" else None
+    got = attention.cross_attention(q, k, v, key_mask=bias, scale=1.0).double()
+    logit = torch.einsum("bqhd,bkhd->bhqk", q[..., :1].double(), k[..., :1].double().repeat_interleave(h // hk, 2))
+    if bias is not None:
+        logit = logit + bias.double()[:, None, None]
+    w = torch.softmax(logit, -1)
+    z = v.double().repeat_interleave(h // hk, 2).permute(0, 2, 1, 3)
+    want, mass = ((w @ x).transpose(1, 2) for x in (z, z.abs()))
+    eps, half_step = 2.0**-11, 2.0**-25
+    tol = (eps * 1.01 + 2 * 20 * 2.0**-21 + 2.0**-20) * mass + eps * 1.01 * want.abs() + half_step \
+        + 2.0**-32 * z.abs().sum(2)[:, None]
+    err = (got - want).abs()
+    assert torch.all(err <= tol), f"worst {float((err / tol).max()):.3f} of the tolerance"
+    assert float((tol / mass).median()) < 0.1   # the tolerance does tell the tail from nothing

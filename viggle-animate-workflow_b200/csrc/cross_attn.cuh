@@ -111,6 +111,13 @@ __global__ void __launch_bounds__(1024) bias_kernel(const void* __restrict__ mas
 // ---------------------------------------------------------------- shared by both kernels
 constexpr int BM = 128, BN = KEY_TILE;  // rows and keys of a tile
 constexpr float GROWTH = 8.0f;          // base-2 growth of a row's maximum that is let stand
+// What is kept as a row's maximum, the m of its weights 2^(y - m), is less than the true one by HEADROOM. The
+// weights of the largest keys are then up to 2^(HEADROOM + GROWTH), which is 2^15 in fp16 (largest 65504), and the
+// smallest that fp16 can hold is 2^-24 / 2^HEADROOM of the largest: with m the maximum itself, a tail of 10^5 keys that
+// are 2^-25 of one dominant key each was lost from the second product while the sum still had it. bf16 has the
+// exponents of fp32 and needs none. Sums and output carry the same factor 2^HEADROOM, pieces too, and it divides out.
+template <typename T>
+constexpr float HEADROOM = std::is_same<T, __half>::value ? 7.0f : 0.0f;
 constexpr int SOFTMAX_WARPS = 16;
 constexpr int WARPS = SOFTMAX_WARPS + 4, THREADS = 32 * WARPS;
 // Registers: 96 a thread at launch, of which the softmax warps take 104 and the last warpgroup leaves
@@ -193,7 +200,11 @@ __device__ __forceinline__ uint32_t pack2<__half>(float lo, float hi) {
   return *reinterpret_cast<const uint32_t*>(&h);
 }
 
-// Base-2 weights of 32 keys: w = 2^(y sc + off), summed in fp32, packed to the type of v.
+// Base-2 weights of 32 keys: w = 2^(y sc + off), summed in fp32, packed to the type of v: both operands of a
+// 16-bit MMA have one type, and weights of 32 bits would take a tf32 copy of v, or a second product for what the
+// rounding leaves. It costs half a step of a weight, 2^-9 (bf16) or 2^-12 (fp16) of it, independent from key to key:
+// the error against 64 bits is 2.2e-3 instead of the 1.7e-3 of the result's own rounding in bf16, 2.4e-4 instead of
+// 2.1e-4 in fp16 (2-norm, normal inputs).
 template <typename T>
 __device__ __forceinline__ float2 weights(const float* y, float sc, float off, uint32_t (&w)[16]) {
   const float2 sc2 = make_float2(sc, sc), off2 = make_float2(off, off);
@@ -220,6 +231,14 @@ __device__ __forceinline__ float max_of(const float* y) {
   for (int u = 0; u < 4; ++u) mx[u] = fmaxf(mx[u], y[N - 4 + u]);
   return fmaxf(fmax3(mx[0], mx[1], mx[2]), mx[3]);
 }
+
+// The largest score of some keys as a row's maximum is kept, and whether it has outgrown the maximum m in use. The
+// latter is the exponent of its weight, rounded as there: no weight passes 2^(HEADROOM + GROWTH) even where the
+// logits are so large that their own steps count.
+template <typename T>
+__device__ __forceinline__ float as_top(float peak, float sc) { return fmaf(peak, sc, -HEADROOM<T>); }
+template <typename T>
+__device__ __forceinline__ bool outgrown(float peak, float sc, float m) { return fmaf(peak, sc, -m) > HEADROOM<T> + GROWTH; }
 
 // Which of the keys key0 + [first, first + 32 W) take part, one bit each, and whether key0 + row does. With
 // a bias only what lies behind the last key is left out here.

@@ -411,7 +411,7 @@ narrow_kernel(const __grid_constant__ CUtensorMap tq, const __grid_constant__ CU
 #pragma unroll 1
           while (true) {
             if (fresh) {
-              const float4 tops = exchange(max_of<32>(y) * sc);
+              const float4 tops = exchange(as_top<T>(max_of<32>(y), sc));
               const float m_new = fmaxf(m, fmaxf(fmaxf(tops.x, tops.y), fmaxf(tops.z, tops.w)));
               if (c.j > 0) {
                 wait_s(g + 1);  // P_{g-1} V_{g-1} done
@@ -425,7 +425,7 @@ narrow_kernel(const __grid_constant__ CUtensorMap tq, const __grid_constant__ CU
             add = weights<T>(y, sc, m == -INFINITY ? 0.0f : -m, w);
             tmem_st_32x32b_x16(t_lane + col_p(g) + 16 * part, w);
             if (fresh) break;
-            fresh = named_barrier_any(1 + quarter, 128, real && max_of<32>(y) * sc > m + GROWTH);
+            fresh = named_barrier_any(1 + quarter, 128, real && outgrown<T>(max_of<32>(y), sc, m));
             if (!fresh) break;
             tmem_st_wait();  // stores are not ordered: these weights have landed before the next go over them
           }

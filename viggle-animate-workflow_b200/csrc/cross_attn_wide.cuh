@@ -12,7 +12,7 @@ namespace wide {
 //   warps 0..7, 8..15  softmax of tile 0 / 1, half a row (64 keys) a thread: scores from TMEM, weights
 //                2^(s scale2 + bias - m) packed to 16 bits over the scores, where the second product reads
 //                them. m is only changed, and O and the sums rescaled, when some row's maximum has grown by
-//                more than 2^8 over it (weights stay below 2^8, sums and O are fp32), which is rare after an
+//                more than 2^8 over it (weights stay in the range of their type, sums and O are fp32), which is rare after an
 //                item's first step.
 //   warp 16      TMA: queries, keys and values in the order of their use
 //   warp 17      the MMAs: S_t = Q_t K_0^T, then per step and tile O_t += P_t V_j followed at once by
@@ -332,10 +332,11 @@ wide_kernel(const __grid_constant__ CUtensorMap tq, const __grid_constant__ CUte
         reg_dep32(*reinterpret_cast<uint32_t(*)[32]>(r + 32));
         float(&y)[64] = reinterpret_cast<float(&)[64]>(r);
         mask_scores<BIAS, 64>(p, it.b, key0, 64 * half, bits, y);
-        const float own = max_of<64>(y) * sc;
+        const float peak = max_of<64>(y);
         // (the barrier also tells that both halves have read the scores that the weights go over)
         tc_fence_before();
-        if (j == 0 || named_barrier_any(pair, 64, real && own > m + GROWTH)) {
+        if (j == 0 || named_barrier_any(pair, 64, real && outgrown<T>(peak, sc, m))) {
+          const float own = as_top<T>(peak, sc);
           const float m_new = fmaxf(m, fmaxf(own, other(own)));
           if (j > 0) {  // O holds P_0 V_0 + ... + P_{j-1} V_{j-1} (done before S_j)
             const float alpha = m_new == -INFINITY ? 1.0f : ex2_approx(m - m_new);
