@@ -109,3 +109,19 @@ def test_a_long_tail_behind_one_key_that_takes_nearly_all(cuda, shape, at, kind)
     err = (got - want).abs()
     assert torch.all(err <= tol), f"worst {float((err / tol).max()):.3f} of the tolerance"
     assert float((tol / mass).median()) < 0.1   # the tolerance does tell the tail from nothing
+
+
+@pytest.mark.parametrize("dtype", ["bf16", "f16"])
+@pytest.mark.parametrize("shape", [NARROW[0], PIECES[0], WIDE[1]])
+def test_logits_whose_own_steps_exceed_one_give_an_average_still(cuda, shape, dtype):
+    """Logits of 10^7 and more, which 32 bits hold to a whole number at best: every result is an average of values
+    all the same, within the roundings of its weights and of itself."""
+    q, k, v = inputs(cuda, dtype, *shape)
+    q, k = (q.float() * 500).to(q.dtype), (k.float() * 1000).to(k.dtype)
+    out = attention.cross_attention(q, k, v, scale=1.0).double()
+    most = v.double().abs().amax(1).repeat_interleave(shape[3] // shape[4], 1)[:, None] * (1 + 2 * torch.finfo(q.dtype).eps)
+    assert bool((out.abs() <= most).all())
+    # a far larger score than any other takes all
+    k[:, 5] = k[:, 5].abs() + 20000
+    out = attention.cross_attention(q.abs(), k, v, scale=1.0)
+    assert torch.equal(out, v[:, 5:6].repeat_interleave(shape[3] // shape[4], 2).expand_as(out))

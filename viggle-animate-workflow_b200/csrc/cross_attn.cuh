@@ -200,6 +200,23 @@ __device__ __forceinline__ uint32_t pack2<__half>(float lo, float hi) {
   return *reinterpret_cast<const uint32_t*>(&h);
 }
 
+// Logits so large that their steps in fp32 come near 1. The weights' exponent y sc - m is formed in one rounding, while
+// m = y sc of the largest key was rounded by itself: its weight is 2^0 only up to half a step of m, which from 2^30 on
+// leaves the range of fp32. There the logits are rounded before m is taken off, as by a product and a subtraction.
+constexpr float LARGE = 4194304.0f;  // 2^22: half a step is a quarter
+template <int N>
+__device__ __forceinline__ float scale_if_large(float (&y)[N], float peak, float& sc) {
+  const bool large = fabsf(peak) * sc > LARGE && peak != -INFINITY;
+  if (__any_sync(0xffffffffu, large)) {
+    const float factor = large ? sc : 1.0f;  // this thread's row goes by its own scores
+#pragma unroll
+    for (int e = 0; e < N; ++e) y[e] *= factor;
+    peak *= factor;
+    if (large) sc = 1.0f;
+  }
+  return peak;
+}
+
 // Base-2 weights of 32 keys: w = 2^(y sc + off), summed in fp32, packed to the type of v: both operands of a
 // 16-bit MMA have one type, and weights of 32 bits would take a tf32 copy of v, or a second product for what the
 // rounding leaves. It costs half a step of a weight, 2^-9 (bf16) or 2^-12 (fp16) of it, independent from key to key:

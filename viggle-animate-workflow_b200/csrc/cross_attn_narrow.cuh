@@ -276,7 +276,7 @@ narrow_kernel(const __grid_constant__ CUtensorMap tq, const __grid_constant__ CU
     const int row = quarter * 32 + lane;
     const uint32_t t_lane = tmem + (static_cast<uint32_t>(quarter * 32) << 16);
     const uint32_t t_o = t_lane + COL_O + part * L::OUT_COLS;
-    const float sc = BIAS ? 1.0f : p.scale2;
+    const float scale = BIAS ? 1.0f : p.scale2;
     // few rows: warps whose rows do not exist only keep step
     const bool live = quarter * 32 < p.rows;
     // 128 rows need not be a whole number of tokens: what is left in the others has no say in rescaling
@@ -404,6 +404,8 @@ narrow_kernel(const __grid_constant__ CUtensorMap tq, const __grid_constant__ CU
           reg_dep32(r);
           float(&y)[32] = reinterpret_cast<float(&)[32]>(r);
           mask_scores<BIAS, 32>(p, c.it.b, key0, 32 * part, bits, y);
+          float sc = scale;
+          const float peak = BIAS ? max_of<32>(y) : scale_if_large(y, max_of<32>(y), sc);
           // Weights with the maximum in use, and once more with a new one if some row's has grown too far
           // (an item's first step has none to start with).
           bool fresh = c.j == 0;
@@ -411,7 +413,7 @@ narrow_kernel(const __grid_constant__ CUtensorMap tq, const __grid_constant__ CU
 #pragma unroll 1
           while (true) {
             if (fresh) {
-              const float4 tops = exchange(as_top<T>(max_of<32>(y), sc));
+              const float4 tops = exchange(as_top<T>(peak, sc));
               const float m_new = fmaxf(m, fmaxf(fmaxf(tops.x, tops.y), fmaxf(tops.z, tops.w)));
               if (c.j > 0) {
                 wait_s(g + 1);  // P_{g-1} V_{g-1} done
@@ -425,7 +427,7 @@ narrow_kernel(const __grid_constant__ CUtensorMap tq, const __grid_constant__ CU
             add = weights<T>(y, sc, m == -INFINITY ? 0.0f : -m, w);
             tmem_st_32x32b_x16(t_lane + col_p(g) + 16 * part, w);
             if (fresh) break;
-            fresh = named_barrier_any(1 + quarter, 128, real && outgrown<T>(max_of<32>(y), sc, m));
+            fresh = named_barrier_any(1 + quarter, 128, real && outgrown<T>(peak, sc, m));
             if (!fresh) break;
             tmem_st_wait();  // stores are not ordered: these weights have landed before the next go over them
           }

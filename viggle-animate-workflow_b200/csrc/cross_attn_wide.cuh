@@ -282,7 +282,7 @@ wide_kernel(const __grid_constant__ CUtensorMap tq, const __grid_constant__ CUte
     const int pair = 1 + 4 * t + quarter;  // barrier of a row's two halves
     const uint32_t t_lane = tmem + (static_cast<uint32_t>(quarter * 32) << 16);
     const uint32_t t_s = t_lane + col_s(t), t_o = t_lane + col_o(t) + half * (DP / 2);
-    const float sc = BIAS ? 1.0f : p.scale2;
+    const float scale = BIAS ? 1.0f : p.scale2;
     // 128 rows need not be a whole number of tokens: what is left in the others has no say in rescaling
     const bool real = row < p.group * p.tokens;
     // After a wait that failed the warp goes through its steps without work (every further wait fails at
@@ -332,7 +332,8 @@ wide_kernel(const __grid_constant__ CUtensorMap tq, const __grid_constant__ CUte
         reg_dep32(*reinterpret_cast<uint32_t(*)[32]>(r + 32));
         float(&y)[64] = reinterpret_cast<float(&)[64]>(r);
         mask_scores<BIAS, 64>(p, it.b, key0, 64 * half, bits, y);
-        const float peak = max_of<64>(y);
+        float sc = scale;
+        const float peak = BIAS ? max_of<64>(y) : scale_if_large(y, max_of<64>(y), sc);
         // (the barrier also tells that both halves have read the scores that the weights go over)
         tc_fence_before();
         if (j == 0 || named_barrier_any(pair, 64, real && outgrown<T>(peak, sc, m))) {
