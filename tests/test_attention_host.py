@@ -187,3 +187,17 @@ def test_oracle_pinned_to_reference_quantiser_golden():
             assert np.array_equal(scales.view(np.uint32), data[f"{key}_{name}_scales"].view(np.uint32)), (key, name)
         _, amax = oa.quant_v(v)
         assert np.float32(amax) == data[f"{key}_v_amax"][0], key
+
+
+def test_the_module_is_importable_without_torch():
+    """Configuration and names only: what needs torch imports it when called."""
+    import subprocess
+    import sys
+    from pathlib import Path
+
+    package = Path(__file__).resolve().parent.parent / "viggle-animate-workflow_b200"
+    code = ("import sys; sys.modules['torch'] = None; sys.path.insert(0, sys.argv[1]); from slimdit import attention as a; "
+            "print(a.TritonAttnConfig().min_seq, a.attn_scale(128, True) > 0, callable(a.cross_attention))")
+    done = subprocess.run([sys.executable, "-c", code, str(package)], capture_output=True, text=True, timeout=120)
+    assert done.returncode == 0, done.stderr[-500:]
+    assert done.stdout.split() == ["12000", "True", "True"]

@@ -23,16 +23,13 @@ from __future__ import annotations
 
 import ctypes
 import dataclasses
+import functools
 import time
 
-import torch
-
 from . import _native as nat
-from .ops import _no_grad, _view
 
 DEFAULT_MIN_SEQ = 12000  # below this the dense path wins outright (attention_triton.py:34)
 HEAD_DIM = 128  # the one head dim the kernel supports (MiniMax-H3: 56 heads x 128)
-_MASK_TYPES = {torch.float32: nat.F32, torch.bfloat16: nat.BF16, torch.float16: nat.F16, torch.bool: nat.MASK_BOOL}
 
 
 def unwrap(value):
@@ -241,9 +238,21 @@ def attention_heads(qkv, heads: int, rank: int, world: int, rotate: bool = True,
     return out
 
 
+@functools.cache
+def _torch_parts():
+    """torch and what of this package needs it: the module itself can be imported without."""
+    import torch
+
+    from .ops import _no_grad, _view
+
+    types = {torch.float32: nat.F32, torch.bfloat16: nat.BF16, torch.float16: nat.F16, torch.bool: nat.MASK_BOOL}
+    return torch, types, _no_grad, _view
+
+
 def _cross_rows(t, name: str, shared: bool):
     """[S, H, D] or [B, S, H, D] as a 4-D view of 16-byte aligned rows (copied when it is not one);
     ``shared``: strides of 0 may stay for the batch and the heads."""
+    torch = _torch_parts()[0]
     if not isinstance(t, torch.Tensor) or not t.is_cuda:
         nat.require_cuda()
         raise TypeError(f"{name} must be a CUDA tensor")
@@ -276,6 +285,7 @@ def cross_attention(q, k, v, key_mask=None, kv_lengths=None, scale: float | None
     apply. What stands in excluded keys and values, NaN included, has no influence; a row without keys
     is 0. scale: D^-0.5 if not given. Scores, maxima and sums are fp32; the weights are rounded to the
     type of v for the second product. Inference only: there is no backward pass."""
+    torch, mask_types, _no_grad, _view = _torch_parts()
     q4, k4, v4 = _cross_rows(q, "q", False), _cross_rows(k, "k", True), _cross_rows(v, "v", True)
     _no_grad(q, k, v, key_mask)
     if k.dim() != q.dim() or v.dim() != q.dim():
@@ -289,7 +299,7 @@ def cross_attention(q, k, v, key_mask=None, kv_lengths=None, scale: float | None
         raise ValueError(f"k {tuple(k.shape)} and v {tuple(v.shape)} do not fit q {tuple(q.shape)}")
     mask_ptr, mask_type, mask_b, mask_k, additive = None, 0, 0, 0, 0
     if key_mask is not None:
-        if not isinstance(key_mask, torch.Tensor) or key_mask.dtype not in _MASK_TYPES:
+        if not isinstance(key_mask, torch.Tensor) or key_mask.dtype not in mask_types:
             raise TypeError("key_mask must be a bool, fp32, bf16 or fp16 tensor")
         if key_mask.device != dev:
             raise ValueError("key_mask must be on the device of q")
@@ -297,7 +307,7 @@ def cross_attention(q, k, v, key_mask=None, kv_lengths=None, scale: float | None
         if not 1 <= m.dim() <= 2 or m.shape[-1] != sk or (m.dim() == 2 and m.shape[0] not in (1, b)):
             raise ValueError(f"key_mask {tuple(key_mask.shape)} does not fit {b} x {sk} keys (masks per query are not "
                              "supported)")
-        mask_ptr, mask_type, mask_k = m.data_ptr(), _MASK_TYPES[m.dtype], m.stride(-1)
+        mask_ptr, mask_type, mask_k = m.data_ptr(), mask_types[m.dtype], m.stride(-1)
         mask_b = m.stride(0) if m.dim() == 2 and m.shape[0] == b and b > 1 else 0
         additive = 1 if mask_type != nat.MASK_BOOL else 0
     len_ptr, len_bits = None, 0
