@@ -93,3 +93,21 @@ def test_the_c_entry_refuses_before_any_device_work():
     assert call(pos=None) == _native.SLIM_ERR_NULL
     assert call(seq=0) == _native.SLIM_OK
     assert call(batch=0, q=None) == _native.SLIM_OK
+
+
+def test_tensors_that_expect_a_derivative_are_refused():
+    from torch.autograd import forward_ad
+
+    x = torch.zeros(3)
+    ops._no_grad(x, None, 1.0)
+    with pytest.raises(ValueError, match="backward"):
+        ops._no_grad(None, x.clone().requires_grad_())
+    with torch.no_grad():
+        ops._no_grad(x.clone().requires_grad_())
+        with forward_ad.dual_level():   # which no_grad does not close
+            dual = forward_ad.make_dual(x, torch.ones(3))
+            ops._no_grad(x, dual.detach())
+            with pytest.raises(ValueError, match="forward"):
+                ops._no_grad(x, dual)
+    with pytest.raises(ValueError, match="forward"):
+        torch.func.jvp(lambda t: (ops._no_grad(t), t)[1], (x,), (x,))

@@ -287,7 +287,7 @@ def cross_attention(q, k, v, key_mask=None, kv_lengths=None, scale: float | None
     type of v for the second product. Inference only: there is no backward pass."""
     torch, mask_types, _no_grad, _view = _torch_parts()
     q4, k4, v4 = _cross_rows(q, "q", False), _cross_rows(k, "k", True), _cross_rows(v, "v", True)
-    _no_grad(q, k, v, key_mask)
+    _no_grad(q, k, v, key_mask, scale)
     if k.dim() != q.dim() or v.dim() != q.dim():
         raise ValueError("q, k and v must have the same number of dimensions")
     b, sq, h, d = q4.shape

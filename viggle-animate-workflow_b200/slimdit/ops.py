@@ -23,6 +23,7 @@ computation runs in libslimdit_b200.so).
 from __future__ import annotations
 
 import torch
+from torch.autograd import forward_ad
 
 from . import _native as nat
 
@@ -525,7 +526,11 @@ _LAYOUTS = {"half": nat.ROTARY_HALF, "interleaved": nat.ROTARY_INTERLEAVED}
 
 
 def _no_grad(*tensors) -> None:
-    """The kernels record no gradient: refuse tensors that expect one instead of dropping it."""
+    """The kernels record no gradient and carry no tangent: refuse tensors that expect one instead of dropping it."""
+    if getattr(forward_ad, "_current_level", 0) >= 0:  # a forward-mode level is open, under no_grad too
+        for t in tensors:
+            if isinstance(t, torch.Tensor) and forward_ad.unpack_dual(t).tangent is not None:
+                raise ValueError("this operator has no forward-mode derivative; detach its inputs")
     if not torch.is_grad_enabled():
         return
     for t in tensors:
@@ -599,11 +604,12 @@ def rotary(q: torch.Tensor, k: torch.Tensor | None, positions: torch.Tensor, inv
     magnitude is ``magnitude``. layout "half" pairs elements j and j + R/2, "interleaved" 2j and
     2j + 1. ``inverse`` turns by the opposite angles (with 1/magnitude it undoes the rotation).
     Returns (q', k'), or q' alone when k is None: new contiguous tensors, or q and k themselves with
-    ``inplace``. The angle is reduced in fp64, the products are fp32, rounded once."""
+    ``inplace``. The angle is reduced in fp64, the products are fp32, rounded once. Inference only: q, k and
+    inv_freq that expect a derivative are refused."""
     if layout not in _LAYOUTS:
         raise ValueError(f"layout must be one of {sorted(_LAYOUTS)}")
     q4 = _rows4(q, "q", inplace)
-    _no_grad(q, k)
+    _no_grad(q, k, inv_freq)
     b, s, h, d = q4.shape
     dev, dtype = q4.device, q4.dtype
     k4, hk = None, 0
