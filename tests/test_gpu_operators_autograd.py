@@ -44,3 +44,26 @@ def test_forward_mode_duals_are_refused(cuda, qkv, which):
             with pytest.raises(ValueError, match="forward"):
                 ops.rotary(*turned, inplace=inplace)
             assert torch.equal(qkv[0], before)
+
+
+def test_a_rotation_in_place_is_seen_by_autograd(cuda, qkv):
+    q, k, _ = qkv
+    pos, freq = torch.arange(6, device=cuda), torch.rand(32, device=cuda)
+    w = torch.ones(64, device=cuda, dtype=q.dtype, requires_grad=True)
+    versions = q._version, k._version
+    with torch.no_grad():
+        ops.rotary(q, k, pos, freq)
+    assert (q._version, k._version) == versions
+    loss = (w * q).sum()                    # saves q
+    ops.rotary(q, k, pos, freq, inplace=True)
+    assert q._version > versions[0] and k._version > versions[1]
+    with pytest.raises(RuntimeError, match="modified by an inplace operation"):
+        loss.backward()
+    loss = (w * k).sum()
+    ops.rotary(k[0], None, pos, freq, inplace=True)   # a view of it, without a batch
+    with pytest.raises(RuntimeError, match="modified by an inplace operation"):
+        loss.backward()
+    with torch.inference_mode():
+        made = torch.ones(1, 6, 2, 64, device=cuda)
+        want = ops.rotary(made, None, pos, freq)
+        assert ops.rotary(made, None, pos, freq, inplace=True) is made and torch.equal(made, want)

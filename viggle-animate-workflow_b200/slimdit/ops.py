@@ -24,6 +24,7 @@ from __future__ import annotations
 
 import torch
 from torch.autograd import forward_ad
+from torch.autograd.graph import increment_version
 
 from . import _native as nat
 
@@ -668,6 +669,8 @@ def rotary(q: torch.Tensor, k: torch.Tensor | None, positions: torch.Tensor, inv
                                          freq.data_ptr(), sec, axes, magnitude, 1 if inverse else 0,
                                          nat.raw_stream(dev)))
     if inplace:
+        # written behind autograd's back: what it saved of them must not pass for unchanged
+        increment_version(q if k is None else (q, k))
         return q if k is None else (q, k)
     if q.dim() == 3:
         q_out = q_out[0]
