@@ -37,6 +37,10 @@ def rope_frequencies(rot_dim: int, theta: float = THETA, scaling: str | None = N
     "parts"    by the turns a frequency makes over original_length: up to ``slow`` turns divided by
                factor, from ``fast`` on unchanged, a linear blend between (NTK by parts)
     "yarn"     "parts", with magnitude 0.1 ln(factor) + 1 (Peng et al., "YaRN", 2023)
+
+    The blend is linear in the turns, as that paper defines it. Checkpoints whose code blends linearly in the
+    pair's index between two correction indices were trained with other middle frequencies (the ends agree):
+    their own table belongs in ``inv_freq`` then.
     """
     if rot_dim < 2 or rot_dim % 2:
         raise ValueError(f"the rotated part must be a positive even number, got {rot_dim}")
