@@ -65,3 +65,5 @@ def test_layouts():
     # one row tile a key head: never paired, however many there are
     assert layout(74, 1, 2048, 32, 8, 128)[1:] == layout(75, 1, 2048, 32, 8, 128)[1:] == (1, 16)
     assert layout(4000, 100, 300, 8, 8, 64)[1:] == (1, 3)
+    # many rows: joining pieces of their keys costs more than it saves, few rows: it does not
+    assert layout(2, 200, 4000, 24, 24, 64)[1] == 1 and layout(2, 7, 4000, 24, 24, 64)[1] > 1

@@ -36,10 +36,21 @@ struct Plan {
   int64_t floats;             // of the pieces' results
 };
 
-// The cheapest layout by a count of steps, one row tile x one key tile in the narrow kernel (about 1.25 us).
+// The cheapest layout by a count of steps, one row tile x one key tile in the narrow kernel (1.23 us).
 // The wide kernel takes two row tiles x one key tile in 1.6 of them and moves half the keys and values: it
-// wins as soon as there are enough pairs of row tiles for the SMs. An item's ends cost 1. Pieces cost a
-// second launch and their sums through memory: 6, and one more for every 4 MB.
+// wins as soon as there are enough pairs of row tiles for the SMs. An item's ends cost 1.
+//
+// Pieces cost join_kernel: 2.5 steps, 1 for every 700 rows (a block each) and 1 for every 4 MB of their sums, taken from
+// captured calls at 80 shapes of 1 to 200 queries over 500 to 20000 keys, heads 8 to 32 of 64 and 128. A call outside of
+// a graph also pays a second launch on the host, so they count 6 at least. At 4 x 1 query over 1500 keys x 16 heads of
+// 64 that keeps one launch: 20 us on the device instead of 16 in two pieces, but 20 us a call instead of 26 when calls
+// are issued one by one. 2 x 200 queries over 4000 keys x 24 heads: 47 us unsplit, 58 in three pieces.
+inline double pieces_cost(int64_t s, int64_t tiles, int rows, int dp) {
+  const double join = 2.5 + static_cast<double>(tiles * rows) / 700 +
+                      static_cast<double>(narrow::split_floats(s, tiles, rows, dp)) / (1 << 20);
+  return join > 6.0 ? join : 6.0;
+}
+
 inline Plan make_plan(int64_t batch, int64_t q_len, int64_t kv_len, int heads, int kv_heads, int dim) {
   Plan p{};
   p.group = heads / kv_heads;
@@ -60,7 +71,7 @@ inline Plan make_plan(int64_t batch, int64_t q_len, int64_t kv_len, int heads, i
     const int64_t per = (nk + s - 1) / s;
     if (s > 1 && (s - 1) * per >= nk) continue;  // the last pieces would be empty
     double cost = static_cast<double>((tiles * s + sms - 1) / sms * (per + 1));
-    if (s > 1) cost += 6.0 + static_cast<double>(narrow::split_floats(s, tiles, p.rows, dp)) / (1 << 20);
+    if (s > 1) cost += pieces_cost(s, tiles, p.rows, dp);
     if (cost < best) {
       best = cost;
       p.splits = static_cast<int>(s);
