@@ -136,7 +136,7 @@ wide_kernel(const __grid_constant__ CUtensorMap tq, const __grid_constant__ CUte
           ok = ok && mbar_wait_abort(bar, ph, kErrWaitTimeoutProducer, &sh.abort);
           return ok;
         };
-        Item prev;
+        Item prev{};
         bool any = false;
         // one pair: the values of the step before (prev, step v_step) and the keys of this one
         auto pair = [&](const Item* it, int j, int v_step) {

@@ -96,7 +96,7 @@ __device__ __forceinline__ uint32_t pack2<__half>(float lo, float hi) {
 // P pairs: partners in u and v (HALF), or neighbours in u then v. cs[e * step]: (cos, sin) of pair e.
 template <typename T, int P, bool HALF>
 __device__ __forceinline__ void turn(Vec<T, P>& u, Vec<T, P>& v, const float2* cs, int step) {
-  if constexpr (sizeof(T) == 2 && P >= 2) {  // by words: the kernel is close to being bound by issue
+  if constexpr (sizeof(T) == 2 && P >= 2) {  // by words: the kernel is not far from being bound by issue
     uint32_t* uw = reinterpret_cast<uint32_t*>(&u);
     uint32_t* vw = reinterpret_cast<uint32_t*>(&v);
     if constexpr (HALF) {
@@ -115,16 +115,16 @@ __device__ __forceinline__ void turn(Vec<T, P>& u, Vec<T, P>& v, const float2* c
         word = pack2<T>(turn_x(z.x, z.y, a), turn_y(z.x, z.y, a));
       }
     }
-    return;
-  }
+  } else {
 #pragma unroll
-  for (int e = 0; e < P; ++e) {
-    T& xe = HALF || P == 1 ? u.e[e] : 2 * e < P ? u.e[2 * e % P] : v.e[2 * e % P];
-    T& ye = HALF || P == 1 ? v.e[e] : 2 * e < P ? u.e[(2 * e + 1) % P] : v.e[(2 * e + 1) % P];
-    const float2 a = cs[e * step];
-    const float x = to_f<T>(xe), y = to_f<T>(ye);
-    xe = from_f<T>(turn_x(x, y, a));
-    ye = from_f<T>(turn_y(x, y, a));
+    for (int e = 0; e < P; ++e) {
+      T& xe = HALF || P == 1 ? u.e[e] : 2 * e < P ? u.e[2 * e % P] : v.e[2 * e % P];
+      T& ye = HALF || P == 1 ? v.e[e] : 2 * e < P ? u.e[(2 * e + 1) % P] : v.e[(2 * e + 1) % P];
+      const float2 a = cs[e * step];
+      const float x = to_f<T>(xe), y = to_f<T>(ye);
+      xe = from_f<T>(turn_x(x, y, a));
+      ye = from_f<T>(turn_y(x, y, a));
+    }
   }
 }
 
