@@ -205,8 +205,8 @@ __device__ __forceinline__ uint32_t pack2<__half>(float lo, float hi) {
 // leaves the range of fp32. There the logits are rounded before m is taken off, as by a product and a subtraction.
 constexpr float LARGE = 4194304.0f;  // 2^22: half a step is a quarter
 template <int N>
-__device__ __forceinline__ float scale_if_large(float (&y)[N], float peak, float& sc) {
-  const bool large = fabsf(peak) * sc > LARGE && peak != -INFINITY;
+__device__ __forceinline__ float scale_if_large(float (&y)[N], float peak, bool real, float& sc) {
+  const bool large = real && fabsf(peak) * sc > LARGE && peak != -INFINITY;
   if (__any_sync(0xffffffffu, large)) {
     const float factor = large ? sc : 1.0f;  // this thread's row goes by its own scores
 #pragma unroll

@@ -279,7 +279,7 @@ narrow_kernel(const __grid_constant__ CUtensorMap tq, const __grid_constant__ CU
     const float scale = BIAS ? 1.0f : p.scale2;
     // few rows: warps whose rows do not exist only keep step
     const bool live = quarter * 32 < p.rows;
-    // 128 rows need not be a whole number of tokens: what is left in the others has no say in rescaling
+    // 128 rows need not be a whole number of tokens: what is left in the others has no say in what is done for all
     const bool real = row < p.group * p.tokens;
     // After a wait that failed the warp goes through its steps without work (every further wait fails at
     // once), so that a row's four warps meet at each of their barriers.
@@ -405,7 +405,7 @@ narrow_kernel(const __grid_constant__ CUtensorMap tq, const __grid_constant__ CU
           float(&y)[32] = reinterpret_cast<float(&)[32]>(r);
           mask_scores<BIAS, 32>(p, c.it.b, key0, 32 * part, bits, y);
           float sc = scale;
-          const float peak = BIAS ? max_of<32>(y) : scale_if_large(y, max_of<32>(y), sc);
+          const float peak = BIAS ? max_of<32>(y) : scale_if_large(y, max_of<32>(y), real, sc);
           // Weights with the maximum in use, and once more with a new one if some row's has grown too far
           // (an item's first step has none to start with).
           bool fresh = c.j == 0;

@@ -283,7 +283,7 @@ wide_kernel(const __grid_constant__ CUtensorMap tq, const __grid_constant__ CUte
     const uint32_t t_lane = tmem + (static_cast<uint32_t>(quarter * 32) << 16);
     const uint32_t t_s = t_lane + col_s(t), t_o = t_lane + col_o(t) + half * (DP / 2);
     const float scale = BIAS ? 1.0f : p.scale2;
-    // 128 rows need not be a whole number of tokens: what is left in the others has no say in rescaling
+    // 128 rows need not be a whole number of tokens: what is left in the others has no say in what is done for all
     const bool real = row < p.group * p.tokens;
     // After a wait that failed the warp goes through its steps without work (every further wait fails at
     // once), so that both halves meet at each of their barriers.
@@ -333,7 +333,7 @@ wide_kernel(const __grid_constant__ CUtensorMap tq, const __grid_constant__ CUte
         float(&y)[64] = reinterpret_cast<float(&)[64]>(r);
         mask_scores<BIAS, 64>(p, it.b, key0, 64 * half, bits, y);
         float sc = scale;
-        const float peak = BIAS ? max_of<64>(y) : scale_if_large(y, max_of<64>(y), sc);
+        const float peak = BIAS ? max_of<64>(y) : scale_if_large(y, max_of<64>(y), real, sc);
         // (the barrier also tells that both halves have read the scores that the weights go over)
         tc_fence_before();
         if (j == 0 || named_barrier_any(pair, 64, real && outgrown<T>(peak, sc, m))) {
