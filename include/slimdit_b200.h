@@ -331,7 +331,7 @@ int slim_rotary(const slim_view* q, const slim_view* q_out, int heads_q, const s
  * out = softmax(scale * q k^T + bias) v. q, out: [batch, q_len, heads, dim]; k, v: [batch, kv_len,
  * kv_heads, dim] (heads a multiple of kv_heads, at most 128 to one), bf16 or fp16, rows 16-byte
  * aligned; dim a multiple of 8 up to 128; strides positive, but k and v may have a batch or head
- * stride of 0 (shared by the sequences or heads). Scores, maxima and sums are fp32. */
+ * stride of 0 (shared by the sequences or heads); scale positive. Scores, maxima and sums are fp32. */
 #define SLIM_MASK_BOOL 3 /* bytes: nonzero = the key takes part */
 
 /* Bytes of the workspace of slim_cross_attn; additive != 0 when an additive mask is given. */

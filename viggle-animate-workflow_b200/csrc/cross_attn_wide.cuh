@@ -12,7 +12,7 @@ namespace wide {
 //   warps 0..7, 8..15  softmax of tile 0 / 1, half a row (64 keys) a thread: scores from TMEM, weights
 //                2^(s scale2 + bias - m) packed to 16 bits over the scores, where the second product reads
 //                them. m is only changed, and O and the sums rescaled, when some row's maximum has grown by
-//                more than 2^8 over it (weights stay in the range of their type, sums and O are fp32), which is rare after an
+//                more than 2^8 over it (so weights stay in their type's range; sums and O are fp32), which is rare after an
 //                item's first step.
 //   warp 16      TMA: queries, keys and values in the order of their use
 //   warp 17      the MMAs: S_t = Q_t K_0^T, then per step and tile O_t += P_t V_j followed at once by
@@ -22,7 +22,8 @@ namespace wide {
 //   warp 18      hands loads that are done with back to the producer
 // Excluded keys have weight 0; their rows of V are cleared in shared memory, as 0 * NaN is not 0.
 //
-// 16384 x 16111 x 24 heads of 128, bf16: 2.67 ms, 1210 TFLOP/s. A step (both tiles) takes 3900 cycles: the
+// 16384 x 16111 x 24 heads of 128, bf16: 2.66 to 2.78 ms in single launches (1170 to 1220 TFLOP/s, by the card), 3.1 ms
+// (1050) one after the other under the power cap. A step (both tiles) takes 3900 cycles: the
 // products alone 2700 of them (their operands come through shared memory), the exponentials alone 2050,
 // and a tile's scores -> weights -> second product -> next scores chain 3900, which bounds it now. A row a
 // thread instead of half a row: 2.79 ms.

@@ -10,8 +10,9 @@
 // fp64, because pos * inv_freq in fp32 is off by up to 2^-24 of the whole angle, not of a turn),
 // then all heads of q and k go through in 16-byte accesses. The products and sums are fp32,
 // rounded once to the element type. 30026 tokens x 112 heads x 128, 96 of them turned, bf16 rows of
-// a packed buffer: 272 us, 6.3 TB/s; by single elements instead of words it took 293 us, as the
-// kernel is then close to being bound by instruction issue (70 % of the slots).
+// a packed buffer: 272 us in a single launch (6.3 TB/s), 275 to 281 one call after the other (6.1 to
+// 6.3), 256 in place; by single elements instead of words a single launch took 293 us, as the kernel is then close
+// to being bound by instruction issue (70 % of the slots, by words 63 %).
 #include <cuda_bf16.h>
 #include <cuda_fp16.h>
 #include <cuda_runtime.h>
@@ -175,7 +176,7 @@ __global__ void __launch_bounds__(THREADS, BLOCKS) rotary_kernel(const Params p)
 
   // Rows of this block: (token, head); this thread takes chunk c of every rows_step-th. (Two or four rows
   // in flight a thread cost more in registers, hence threads, than they gain: 293, 381, 625 us at 30026
-  // tokens x 112 heads x 128.)
+  // tokens x 112 heads x 128, in the form by single elements.)
   const int rows_step = THREADS / p.chunks > 0 ? THREADS / p.chunks : 1;
   for (int c = threadIdx.x % p.chunks; c < p.chunks; c += THREADS) {
     const int row0 = threadIdx.x / p.chunks;
@@ -241,10 +242,10 @@ cudaError_t launch(Params& p, bool half, bool copies, cudaStream_t st) {
   }
   p.rot_chunks = p.pairs / P;
   p.chunks = p.rot_chunks + (copies ? (p.dim - p.rot) / P : 0);
-  // Tokens per block: up to twelve rounds of its threads, so that the table's latency is a small part (four
-  // took 14 us more at 30026 tokens x 112 heads x 128), within the table; fewer where that leaves
-  // SMs idle, or a second round of blocks with few in it (8198 tokens x 48 heads: 47 us with two tokens a
-  // block, 51 with five).
+  // Tokens per block: up to twelve rounds of its threads, so that the table's latency is a small part (65537 tokens x
+  // 10 heads of 64 in fp32: 57 us with sixteen, 139 with one; 30026 tokens x 112 heads of 128, bf16: 268 us with three,
+  // 287 with eight), within the table; fewer where that leaves SMs idle, or a second round of blocks with few in it
+  // (8198 tokens x 48 heads of 128: 40 us with two tokens a block, 42 with five).
   const int64_t items = static_cast<int64_t>(p.heads) * p.chunks;
   int64_t tokens = (12 * THREADS + items - 1) / items;
   if (tokens > MAX_TOKENS) tokens = MAX_TOKENS;

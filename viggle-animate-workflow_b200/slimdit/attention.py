@@ -283,7 +283,7 @@ def cross_attention(q, k, v, key_mask=None, kv_lengths=None, scale: float | None
     -inf excludes a key, a finite value, the type's lowest included, is added to its logits.
     kv_lengths: int32 or int64 [B] on the device, keys from there on are excluded; with a mask both
     apply. What stands in excluded keys and values, NaN included, has no influence; a row without keys
-    is 0. scale: D^-0.5 if not given. Scores, maxima and sums are fp32; the weights are rounded to the
+    is 0. scale: positive, D^-0.5 if not given. Scores, maxima and sums are fp32; the weights are rounded to the
     type of v for the second product. Inference only: there is no backward pass."""
     torch, mask_types, _no_grad, _view = _torch_parts()
     q4, k4, v4 = _cross_rows(q, "q", False), _cross_rows(k, "k", True), _cross_rows(v, "v", True)
