@@ -255,7 +255,9 @@ __device__ __forceinline__ float max_of(const float* y) {
 template <typename T>
 __device__ __forceinline__ float as_top(float peak, float sc) { return fmaf(peak, sc, -HEADROOM<T>); }
 template <typename T>
-__device__ __forceinline__ bool outgrown(float peak, float sc, float m) { return fmaf(peak, sc, -m) > HEADROOM<T> + GROWTH; }
+__device__ __forceinline__ bool outgrown(float peak, float sc, float m) {
+  return fmaf(peak, sc, -m) > HEADROOM<T> + GROWTH;
+}
 
 // Which of the keys key0 + [first, first + 32 W) take part, one bit each, and whether key0 + row does. With
 // a bias only what lies behind the last key is left out here.

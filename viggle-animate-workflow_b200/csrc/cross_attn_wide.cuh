@@ -12,8 +12,8 @@ namespace wide {
 //   warps 0..7, 8..15  softmax of tile 0 / 1, half a row (64 keys) a thread: scores from TMEM, weights
 //                2^(s scale2 + bias - m) packed to 16 bits over the scores, where the second product reads
 //                them. m is only changed, and O and the sums rescaled, when some row's maximum has grown by
-//                more than 2^8 over it (so weights stay in their type's range; sums and O are fp32), which is rare after an
-//                item's first step.
+//                more than 2^8 over it (so weights stay in their type's range; sums and O are fp32), which is
+//                rare after an item's first step.
 //   warp 16      TMA: queries, keys and values in the order of their use
 //   warp 17      the MMAs: S_t = Q_t K_0^T, then per step and tile O_t += P_t V_j followed at once by
 //                S_t = Q_t K_{j+1}^T: while one tile is in the softmax the tensor cores work on the other.
